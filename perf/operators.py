@@ -128,17 +128,17 @@ def _lens(case):
     return q, kv
 
 
-def _sections(d):
-    """How the rotation's frequencies are shared out to time, height and width."""
-    half = d // 2
-    t = half // 4
+def _sections(case):
+    """How the rotation's frequencies are shared out to time, height and width; interleaved, time has the most."""
+    half = case["d"] // 2
+    t = 3 * half // 8 if case["interleaved"] else half // 4
     h = (half - t) // 2
     return [t, h, half - t - h]
 
 
 def _axes(case):
     """The axis of every frequency."""
-    half, sec = case["d"] // 2, _sections(case["d"])
+    half, sec = case["d"] // 2, _sections(case)
     if not case["interleaved"]:
         return [a for a in range(3) for _ in range(sec[a])]
     return [j % 3 if j % 3 and j < 3 * sec[j % 3] else 0 for j in range(half)]
@@ -257,7 +257,7 @@ def _prepare_mrope(case, g):
         s["ks"], s["vs"] = (torch.rand((pool, hkv, p), generator=g, device="cuda") * 0.01 for _ in range(2))
     if own:
         package, _ = _library()
-        s["axes"] = package.mrope_axes(_sections(d), interleaved=case["interleaved"])
+        s["axes"] = package.mrope_axes(_sections(case), interleaved=case["interleaved"])
         s["cache"] = package.paged_kv(s["k"], s["v"], table, s["lens"], n_kv_heads=hkv, page_size=p, head_dim=d) \
             if case["bits"] == 16 else package.paged_kv8(s["k"], s["v"], s["ks"], s["vs"], table, s["lens"], n_kv_heads=hkv,
                                                          page_size=p)
