@@ -642,6 +642,67 @@ MF_API mf_status mf_paged_prefill(MfContext *ctx, const MfPagedKv *cache, const 
 MF_API mf_status mf_paged_gather(MfContext *ctx, const MfPagedKv *cache, uint32_t use_v,
                                  uint32_t seq, uint32_t len, void *out);
 
+/* ---- ragged batches of new tokens over a paged cache --------------------------------------
+ * No counterpart in the reference (one sequence, contiguous cache).  A serving step brings every
+ * sequence its own number of new tokens: one that decodes, a few drafted ones to verify, a chunk of
+ * a prompt.  The tokens of all sequences are packed one sequence behind the other; their K/V rows
+ * are in the cache already (mf_paged_mrope_append, mf_paged_kv_append), as the last q_lens[b] of
+ * the kv_lens[b] rows of sequence b.  Row r of sequence b stands at position
+ * p = kv_lens[b] - q_lens[b] + r and sees key k iff
+ *     k <= p  and  (window == 0  or  p - k < window  or  k < n_sinks)
+ * (a sliding window of `window` keys, itself included, and n_sinks first tokens that stay visible).
+ * A row that sees nothing (q_lens[b] > kv_lens[b]) comes out as zeros.
+ *
+ * A plan holds the lengths, the work list and the scratch of one such step; it is made from host
+ * lengths, is reused by every layer with this geometry and this window, and is updated in place for
+ * the next step.  max_tokens: the most new tokens of a later update (0: no more than now); the plan
+ * allocates at creation only.  Updates are enqueued on the context's stream; launches that use one
+ * plan must not overlap on the GPU (its partial results and tickets are shared by them), whether
+ * eager or replayed.  A launch captured into a CUDA graph follows the updates made before its
+ * replay; an update itself is refused while the stream is being captured. */
+typedef struct MfChunkPlan MfChunkPlan;
+MF_API mf_status mf_chunk_plan_create(MfContext *ctx, const uint32_t *q_lens_host, const uint32_t *kv_lens_host,
+                                      uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                                      uint32_t page_size, uint32_t window, uint32_t n_sinks, uint32_t max_tokens,
+                                      MfChunkPlan **out);
+MF_API mf_status mf_chunk_plan_update(MfContext *ctx, MfChunkPlan *plan, const uint32_t *q_lens_host,
+                                      const uint32_t *kv_lens_host);
+MF_API void mf_chunk_plan_destroy(MfContext *ctx, MfChunkPlan *plan);
+MF_API uint32_t mf_chunk_plan_tokens(const MfChunkPlan *plan);
+/* q and out: f16, 16-byte aligned; element (token t, head h, dim d) at t * stride_t + h * stride_h + d,
+ * strides in elements, multiples of 8.  q is rotated already.  scale >= 0. */
+typedef struct MfPagedChunkArgs {
+    const void *q;
+    void *out;
+    uint64_t q_stride_t, q_stride_h, out_stride_t, out_stride_h;
+    float scale;
+} MfPagedChunkArgs;
+/* Attention of the plan's step over the pages of its sequences (cache->kv_lens is not read: the plan has
+ * the lengths).  Page-table entries of pages that no row sees are not read: they may have been given
+ * back (mf_page_pool_release_hidden).  head_dim 64 or 128, pages of 8 to 128 rows (a power of two),
+ * up to 64 query heads per kv head. */
+MF_API mf_status mf_paged_chunk_attention(MfContext *ctx, const MfChunkPlan *plan, const MfPagedKv *cache,
+                                          const MfPagedChunkArgs *args);
+
+/* Append of a ragged batch with rotary positions on several axes (text and images or video: time,
+ * height, width).  No counterpart in the reference.  Token t (packed as above) of sequence b goes to
+ * cache row kv_lens[b] - (q_begin[b + 1] - t); its rotation is another matter: frequency j of a head
+ * (dims j and j + D/2 in MF_ROPE_MODE_NEOX, 2j and 2j + 1 in MF_ROPE_MODE_NORMAL) turns by row
+ * positions[axis[j]][t] of the cos / sin tables.  With equal positions on all axes this is the
+ * rotation of mf_paged_kv_append, bit for bit. */
+#define MF_MAX_ROPE_AXES 4
+typedef struct MfMropeAppendArgs {
+    const void *q, *k, *v;      /* device f16 [tokens, heads * head_dim], rows q/k/v_stride elements apart */
+    void *q_rot;                /* device f16, like q; may be NULL (q is then not read and may be NULL) */
+    const void *cos, *sin;      /* device f16 [table_rows, head_dim/2] */
+    const uint32_t *positions;  /* device [n_axes, position_stride] */
+    const uint32_t *q_begin;    /* device [batch + 1], q_begin[0] = 0, q_begin[batch] = tokens */
+    uint64_t q_stride, k_stride, v_stride, q_rot_stride; /* elements, multiples of 8 */
+    uint32_t tokens, n_heads, n_axes, position_stride, table_rows, rope_mode;
+    uint8_t axis[64];           /* axis of frequency j < head_dim/2 */
+} MfMropeAppendArgs;
+MF_API mf_status mf_paged_mrope_append(MfContext *ctx, const MfPagedKv *cache, const MfMropeAppendArgs *args);
+
 /* Sequence-sharded decode: this shard attends over its own keys only and emits
  * unnormalised f32 partials (acc [batch, Hq, D], m and l [batch, Hq]) for the
  * all-gather + mf_merge_partials step.  kv_lens in `cache` are the shard-local
@@ -689,6 +750,37 @@ MF_API mf_status mf_prefix_cache_lookup(MfPrefixCache *cache, const uint32_t *pr
 /* Copies whole pages (all kv heads, K and V pools) dst_ids[i] <- src_ids[i]; ids are device arrays. */
 MF_API mf_status mf_paged_copy_pages(MfContext *ctx, const MfPagedKv *cache, const uint32_t *src_ids,
                                      const uint32_t *dst_ids, uint32_t n);
+
+/* Pages dst_ids[i] <- src_ids[i] in every layer at once (K and V pools of n_layers caches of one geometry);
+ * the ids are HOST arrays and travel with the launch, so the call needs no upload, keeps nothing and can be
+ * captured.  A source may repeat (several children of one page); a destination may not, nor be a source:
+ * MF_ERR_INVALID_OPERATION before anything moves, as for an id outside the pool. */
+MF_API mf_status mf_paged_move_pages(MfContext *ctx, const MfPagedKv *layers, uint32_t n_layers,
+                                     const uint32_t *src_ids_host, const uint32_t *dst_ids_host, uint32_t n);
+/* A second owner for the first n_tokens tokens of a sequence whose pages are `ids` (ceil(n_tokens /
+ * page_size) of them): full pages are shared (retained), a partly filled last page gets a private copy, since
+ * both owners will write into it.  out_ids: the new owner's pages.  *copy_src / *copy_dst: the copy to be
+ * made (mf_paged_move_pages), or UINT32_MAX each when there is none.  MF_ERR_OUT_OF_MEMORY: no page for
+ * the copy, nothing changed. */
+MF_API mf_status mf_page_pool_fork(MfPagePool *pool, const uint32_t *ids, uint32_t n_tokens, uint32_t page_size,
+                                   uint32_t *out_ids, uint32_t *copy_src, uint32_t *copy_dst);
+/* Gives back the pages of a sequence that no later token sees under a sliding window: kv_len tokens are
+ * cached, the next one stands at position kv_len and sees keys above kv_len - window and the first n_sinks.
+ * ids[i] holds tokens [i * page_size, (i + 1) * page_size); entries given back become UINT32_MAX, entries that
+ * are UINT32_MAX already are passed over.  *released: their number.  window 0: nothing is hidden. */
+MF_API mf_status mf_page_pool_release_hidden(MfPagePool *pool, uint32_t *ids, uint32_t n, uint32_t kv_len,
+                                             uint32_t page_size, uint32_t window, uint32_t n_sinks,
+                                             uint32_t *released);
+/* Renumbers the live pages to [0, live): every live page at or above `live` moves to a free id below it.
+ * src_out / dst_out (capacity cap): the moves, to be made with mf_paged_move_pages before the pool is used
+ * again, and to be applied to every list of ids (mf_remap_page_ids, mf_prefix_cache_remap).  Reference counts
+ * move along.  MF_ERR_OUT_OF_MEMORY: *n_out > cap moves are needed, nothing changed (cap 0 asks). */
+MF_API mf_status mf_page_pool_compact(MfPagePool *pool, uint32_t *src_out, uint32_t *dst_out, uint32_t cap,
+                                      uint32_t *n_out);
+/* ids[i] = dst[j] wherever ids[i] == src[j] (host arrays; no src is a dst). */
+MF_API mf_status mf_remap_page_ids(uint32_t *ids, uint64_t n_ids, const uint32_t *src, const uint32_t *dst, uint32_t n);
+/* The same for the lists that the prefix cache's entries hold. */
+MF_API mf_status mf_prefix_cache_remap(MfPrefixCache *cache, const uint32_t *src, const uint32_t *dst, uint32_t n);
 
 /* ---- 8-bit K/V cache (FP8 E4M3, one f32 scale per cached row) ------------------------
  * The reference has only a roadmap for a quantised cache (docs/FLASH.md:121-186,
@@ -745,6 +837,11 @@ MF_API mf_status mf_paged_kv8_append(MfContext *ctx, const MfPagedKv8 *cache, co
                                      const void *v, void *q_rot, const void *cos, const void *sin, uint32_t n_heads,
                                      uint32_t rope_mode, uint32_t apply_rope, uint32_t seq, uint32_t position_offset,
                                      uint32_t seq_len);
+/* mf_paged_mrope_append for the 8-bit cache: the rotated K rows (rounded to f16) and the V rows are quantised. */
+MF_API mf_status mf_paged_kv8_mrope_append(MfContext *ctx, const MfPagedKv8 *cache, const MfMropeAppendArgs *args);
+/* mf_paged_move_pages for the 8-bit cache: bytes and row scales. */
+MF_API mf_status mf_paged_kv8_move_pages(MfContext *ctx, const MfPagedKv8 *layers, uint32_t n_layers,
+                                         const uint32_t *src_ids_host, const uint32_t *dst_ids_host, uint32_t n);
 /* The first `len` rows of one sequence, dequantised, as a contiguous [n_kv_heads, len, 128] f16 cache. */
 MF_API mf_status mf_paged_kv8_gather(MfContext *ctx, const MfPagedKv8 *cache, uint32_t use_v, uint32_t seq,
                                      uint32_t len, void *out);

@@ -38,6 +38,7 @@ ROPE_MODE_NEOX, ROPE_MODE_NORMAL = 0, 1
 ROUTE_DECODE, ROUTE_PREFILL, ROUTE_PREFILL_SPLITK, ROUTE_REFERENCE = 1, 2, 3, 4
 DTYPE_F16, DTYPE_F32, DTYPE_U32 = 0, 1, 2
 ALL_SEQUENCES = 0xFFFFFFFF
+FREED_PAGE = 0xFFFFFFFF  # entry of a page list whose page was given back (mf_page_pool_release_hidden)
 OPTION_OVERLAP_LAUNCHES, OPTION_DECODE_STAGES, OPTION_PREFILL_IMPL, OPTION_DECODE_CLUSTERS, OPTION_QKV_IMPL = 1, 2, 3, 4, 5
 OPTION_PLAN_ITEM_COST = 6
 OPTION_PUSH_TAGGED = 7
@@ -136,6 +137,18 @@ class MfPagedPrefillArgs(C.Structure):
     _fields_ = [("q", vp), ("out", vp), ("seq", u32), ("q_len", u32), ("kv_len", u32), ("query_offset", u32),
                 ("n_heads", u32), ("q_stride_h", u32), ("q_stride_m", u32), ("out_stride_h", u32), ("out_stride_m", u32),
                 ("scale", C.c_float)]
+
+
+class MfPagedChunkArgs(C.Structure):
+    _fields_ = [("q", vp), ("out", vp), ("q_stride_t", u64), ("q_stride_h", u64), ("out_stride_t", u64), ("out_stride_h", u64),
+                ("scale", C.c_float)]
+
+
+class MfMropeAppendArgs(C.Structure):
+    _fields_ = [("q", vp), ("k", vp), ("v", vp), ("q_rot", vp), ("cos", vp), ("sin", vp), ("positions", vp), ("q_begin", vp),
+                ("q_stride", u64), ("k_stride", u64), ("v_stride", u64), ("q_rot_stride", u64), ("tokens", u32),
+                ("n_heads", u32), ("n_axes", u32), ("position_stride", u32), ("table_rows", u32), ("rope_mode", u32),
+                ("axis", C.c_uint8 * 64)]
 
 
 class MfFusedQkvArgs(C.Structure):
@@ -245,6 +258,20 @@ _SIGNATURES = {
     "mf_prefix_cache_lookup": (C.c_int32, [vp, vp, u32, C.c_char_p, C.POINTER(u32), vp, u32, C.POINTER(u32)]),
     "mf_paged_prefill": (C.c_int32, [vp, C.POINTER(MfPagedKv), C.POINTER(MfPagedPrefillArgs)]),
     "mf_paged_copy_pages": (C.c_int32, [vp, C.POINTER(MfPagedKv), vp, vp, u32]),
+    "mf_chunk_plan_create": (C.c_int32, [vp, vp, vp] + [u32] * 8 + [C.POINTER(vp)]),
+    "mf_chunk_plan_update": (C.c_int32, [vp, vp, vp, vp]),
+    "mf_chunk_plan_destroy": (None, [vp, vp]),
+    "mf_chunk_plan_tokens": (u32, [vp]),
+    "mf_paged_chunk_attention": (C.c_int32, [vp, vp, C.POINTER(MfPagedKv), C.POINTER(MfPagedChunkArgs)]),
+    "mf_paged_mrope_append": (C.c_int32, [vp, C.POINTER(MfPagedKv), C.POINTER(MfMropeAppendArgs)]),
+    "mf_paged_kv8_mrope_append": (C.c_int32, [vp, C.POINTER(MfPagedKv8), C.POINTER(MfMropeAppendArgs)]),
+    "mf_paged_move_pages": (C.c_int32, [vp, vp, u32, vp, vp, u32]),
+    "mf_paged_kv8_move_pages": (C.c_int32, [vp, vp, u32, vp, vp, u32]),
+    "mf_page_pool_fork": (C.c_int32, [vp, vp, u32, u32, vp, C.POINTER(u32), C.POINTER(u32)]),
+    "mf_page_pool_release_hidden": (C.c_int32, [vp, vp, u32, u32, u32, u32, u32, C.POINTER(u32)]),
+    "mf_page_pool_compact": (C.c_int32, [vp, vp, vp, u32, C.POINTER(u32)]),
+    "mf_remap_page_ids": (C.c_int32, [vp, u64, vp, vp, u32]),
+    "mf_prefix_cache_remap": (C.c_int32, [vp, vp, vp, u32]),
     "mf_peer_exchange_create": (C.c_int32, [vp, u32, u32, u32, u32, C.POINTER(MfPeerExchange), vp]),
     "mf_peer_exchange_attach": (C.c_int32, [vp, C.POINTER(MfPeerExchange), u32, vp]),
     "mf_peer_exchange_destroy": (C.c_int32, [vp, C.POINTER(MfPeerExchange)]),
@@ -512,6 +539,58 @@ class Foundry:
         """dst page <- src page for all kv heads of both pools; ids are device int32/uint32 tensors."""
         self.check(lib.mf_paged_copy_pages(self._h, C.byref(cache), _ptr(src_ids), _ptr(dst_ids), n))
 
+    # -- ragged batches of new tokens ------------------------------------------------------
+
+    def chunk_plan(self, q_lens, kv_lens, *, n_heads, n_kv_heads, head_dim, page_size, window=0, sinks=0,
+                   max_tokens=0) -> "ChunkPlan":
+        return ChunkPlan(self, q_lens, kv_lens, n_heads, n_kv_heads, head_dim, page_size, window, sinks, max_tokens)
+
+    def paged_chunk_attention(self, plan: "ChunkPlan", cache: MfPagedKv, q, out, *, scale=None):
+        """Causal (windowed) attention of the plan's new tokens; q and out: f16 [tokens, Hq*D] or [tokens, Hq, D], any
+        token and head strides that are multiples of 8."""
+        d = cache.head_dim
+        _check_rows(q, plan, d, "q")
+        _check_rows(out, plan, d, "out")
+        a = MfPagedChunkArgs(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1) if q.dim() == 3 else d, out.stride(0),
+                             out.stride(1) if out.dim() == 3 else d, 1.0 / math.sqrt(d) if scale is None else scale)
+        self.check(lib.mf_paged_chunk_attention(self._h, plan._h, C.byref(cache), C.byref(a)))
+
+    def paged_mrope_append(self, cache, q, k, v, q_rot, cos, sin, positions, q_begin, axes, *, n_heads,
+                           rope_mode=ROPE_MODE_NEOX):
+        """Rotate q and k of a ragged batch by positions on several axes and append k, v to the pages of an f16 or an
+        8-bit cache.  q, k, v, q_rot: f16 [tokens, heads*D] (rows may be strided; q and q_rot may be None), positions:
+        int32 [n_axes, tokens], q_begin: int32 [batch + 1], axes: the axis of every frequency (see mrope_axes)."""
+        d, tokens = cache.head_dim, k.shape[0]
+        heads = (("q", q, n_heads), ("k", k, cache.n_kv_heads), ("v", v, cache.n_kv_heads), ("q_rot", q_rot, n_heads))
+        for name, x, h in heads:
+            if x is not None and (x.dim() != 2 or x.shape[0] != tokens or x.shape[1] != h * d or x.stride(1) != 1
+                                  or x.element_size() != 2):
+                raise MetalError(2, f"mrope append: {name} must be f16 [{tokens}, {h * d}] with unit column stride")
+        if cos.shape[1] * 2 != d or sin.shape != cos.shape or not (cos.is_contiguous() and sin.is_contiguous()):
+            raise MetalError(2, f"mrope append: cos / sin must be [rows, {d // 2}]")
+        if positions.dim() != 2 or positions.shape[1] != tokens or positions.stride(1) != 1 or positions.element_size() != 4:
+            raise MetalError(2, f"mrope append: positions must be int32 [n_axes, {tokens}]")
+        if q_begin.numel() != cache.batch + 1 or q_begin.element_size() != 4 or not q_begin.is_contiguous():
+            raise MetalError(2, f"mrope append: q_begin must be int32 [{cache.batch + 1}]")
+        if len(axes) != d // 2:
+            raise MetalError(2, f"mrope append: {len(axes)} axes for {d // 2} frequencies")
+        n_axes = positions.shape[0]
+        a = MfMropeAppendArgs(_ptr(q), k.data_ptr(), v.data_ptr(), _ptr(q_rot), cos.data_ptr(), sin.data_ptr(),
+                              positions.data_ptr(), q_begin.data_ptr(), 0 if q is None else q.stride(0), k.stride(0), v.stride(0),
+                              0 if q_rot is None else q_rot.stride(0), tokens, n_heads, n_axes,
+                              positions.stride(0) if n_axes > 1 else tokens, cos.shape[0], rope_mode)
+        C.memmove(a.axis, bytes(axes), len(axes))
+        fn = lib.mf_paged_kv8_mrope_append if isinstance(cache, MfPagedKv8) else lib.mf_paged_mrope_append
+        self.check(fn(self._h, C.byref(cache), C.byref(a)))
+
+    def paged_move_pages(self, layers, src_ids, dst_ids):
+        """Pages dst <- src in all layers (kv_layers of f16 or 8-bit caches); the ids are host arrays (numpy uint32)."""
+        src, dst = np.ascontiguousarray(src_ids, np.uint32), np.ascontiguousarray(dst_ids, np.uint32)
+        if src.size != dst.size:
+            raise MetalError(2, f"move pages: {src.size} sources, {dst.size} destinations")
+        fn = lib.mf_paged_kv8_move_pages if layers._type_ is MfPagedKv8 else lib.mf_paged_move_pages
+        self.check(fn(self._h, layers, len(layers), src.ctypes.data, dst.ctypes.data, src.size))
+
     def paged_kv_append(self, cache: MfPagedKv, q, k, v, q_rot, cos, sin, *, n_heads, rope_mode=ROPE_MODE_NEOX,
                         apply_rope=True, seq=ALL_SEQUENCES, position_offset=0, seq_len=0):
         self.check(lib.mf_paged_kv_append(self._h, C.byref(cache), _ptr(q), _ptr(k), _ptr(v), _ptr(q_rot), _ptr(cos),
@@ -651,6 +730,35 @@ class PagePool:
         ids = np.ascontiguousarray(ids, np.uint32)
         self._check(lib.mf_page_pool_release(self._h, ids.ctypes.data_as(vp), ids.size), "page pool: release of a free page")
 
+    def fork(self, ids, n_tokens: int, page_size: int):
+        """A second owner for the first n_tokens tokens: (its page ids, copies to make as a list of (src, dst))."""
+        ids = np.ascontiguousarray(ids, np.uint32)
+        n = -(-n_tokens // page_size)
+        if ids.size < n:
+            raise MetalError(2, f"page pool: {ids.size} pages for {n_tokens} tokens")
+        out, src, dst = np.empty(n, np.uint32), u32(0), u32(0)
+        self._check(lib.mf_page_pool_fork(self._h, ids.ctypes.data, n_tokens, page_size, out.ctypes.data, C.byref(src), C.byref(dst)),
+                    "page pool: fork")
+        return out, [] if src.value == FREED_PAGE else [(src.value, dst.value)]
+
+    def release_hidden(self, ids, kv_len: int, page_size: int, window: int, sinks: int = 0):
+        """Give back the pages that no later token sees under the window: (ids with FREED_PAGE in their places, count)."""
+        ids = np.array(ids, np.uint32)
+        n = u32(0)
+        self._check(lib.mf_page_pool_release_hidden(self._h, ids.ctypes.data, ids.size, kv_len, page_size, window, sinks, C.byref(n)),
+                    "page pool: release of a free page")
+        return ids, int(n.value)
+
+    def compact(self):
+        """Renumber the live pages to [0, live): (src, dst) of the moves to make and to apply to every id list."""
+        n = u32(0)
+        st = lib.mf_page_pool_compact(self._h, None, None, 0, C.byref(n))
+        src, dst = np.empty(n.value, np.uint32), np.empty(n.value, np.uint32)
+        if n.value:
+            st = lib.mf_page_pool_compact(self._h, src.ctypes.data, dst.ctypes.data, n.value, C.byref(n))
+        self._check(st, "page pool: compact")
+        return src, dst
+
     @property
     def free_count(self) -> int:
         return int(lib.mf_page_pool_free_count(self._h))
@@ -686,6 +794,13 @@ class PrefixCache:
                                        None if key is None else key.encode(), page_ids.ctypes.data_as(vp), page_ids.size)
         if st != 0:
             raise MetalError(st, "prefix cache store")
+
+    def remap(self, src, dst):
+        """Apply the moves of PagePool.compact to the entries' page lists."""
+        src, dst = np.ascontiguousarray(src, np.uint32), np.ascontiguousarray(dst, np.uint32)
+        st = lib.mf_prefix_cache_remap(self._h, src.ctypes.data, dst.ctypes.data, src.size)
+        if st != 0:
+            raise MetalError(st, "prefix cache remap")
 
     def lookup(self, prompt, key: str | None = None):
         """Returns (matched tokens, page ids retained for the caller)."""
@@ -748,6 +863,82 @@ class DecodePlan:
             self.close()
         except Exception:
             pass
+
+
+class ChunkPlan:
+    """Lengths and work list of one step over a ragged batch of new tokens (see mf_chunk_plan_create)."""
+
+    def __init__(self, foundry: Foundry, q_lens, kv_lens, n_heads, n_kv_heads, head_dim, page_size, window, sinks, max_tokens):
+        self._f, self._h = foundry, None
+        ql, kl = self._lens(q_lens, kv_lens)
+        self.batch, self.n_heads = int(ql.size), n_heads
+        h = vp()
+        foundry.check(lib.mf_chunk_plan_create(foundry._h, ql.ctypes.data, kl.ctypes.data, self.batch, n_heads, n_kv_heads,
+                                               head_dim, page_size, window, sinks, max_tokens, C.byref(h)))
+        self._h = h
+        self.tokens = int(ql.sum())
+
+    @staticmethod
+    def _lens(q_lens, kv_lens):
+        ql, kl = np.ascontiguousarray(q_lens, np.uint32), np.ascontiguousarray(kv_lens, np.uint32)
+        if ql.shape != kl.shape or ql.ndim != 1:
+            raise MetalError(2, f"chunk plan: {ql.shape} new-token counts, {kl.shape} lengths")
+        return ql, kl
+
+    def update(self, q_lens, kv_lens):
+        ql, kl = self._lens(q_lens, kv_lens)
+        if ql.size != self.batch:
+            raise MetalError(2, f"chunk plan: {ql.size} sequences, made for {self.batch}")
+        self._f.check(lib.mf_chunk_plan_update(self._f._h, self._h, ql.ctypes.data, kl.ctypes.data))
+        self.tokens = int(ql.sum())
+
+    def close(self):
+        if getattr(self, "_h", None) and getattr(self._f, "_h", None):
+            lib.mf_chunk_plan_destroy(self._f._h, self._h)
+        self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _check_rows(x, plan: ChunkPlan, d: int, name: str):
+    cols = tuple(x.shape[1:])
+    if x.shape[0] < plan.tokens or cols not in ((plan.n_heads * d,), (plan.n_heads, d)) or x.stride(-1) != 1 or x.element_size() != 2:
+        raise MetalError(2, f"paged chunk attention: {name} {tuple(x.shape)} for {plan.tokens} tokens of {plan.n_heads} heads of {d}")
+
+
+def mrope_axes(sections, interleaved: bool = False) -> bytes:
+    """The axis of every frequency: sections[a] frequencies for axis a, one section behind the other, or interleaved:
+    frequency j goes to axis j % n where that axis still has frequencies left (j < n * sections[axis]), else to axis 0
+    (which therefore has to have the most)."""
+    n, half = len(sections), sum(sections)
+    if interleaved:
+        axes = bytes(j % n if j < n * sections[j % n] else 0 for j in range(half))
+        if [axes.count(a) for a in range(n)] != list(sections):
+            raise MetalError(3, f"mrope axes: sections {list(sections)} cannot be interleaved")
+        return axes
+    return bytes(a for a in range(n) for _ in range(sections[a]))
+
+
+def remap_page_ids(ids, src, dst):
+    """`ids` with the moves of PagePool.compact applied (numpy uint32; FREED_PAGE entries stay)."""
+    ids = np.array(ids, np.uint32)
+    src, dst = np.ascontiguousarray(src, np.uint32), np.ascontiguousarray(dst, np.uint32)
+    st = lib.mf_remap_page_ids(ids.ctypes.data, ids.size, src.ctypes.data, dst.ctypes.data, src.size)
+    if st != 0:
+        raise MetalError(st, "remap page ids")
+    return ids
+
+
+def kv_layers(caches):
+    """The caches of a model's layers (all MfPagedKv or all MfPagedKv8) as the array that paged_move_pages takes."""
+    kind = type(caches[0])
+    arr = (kind * len(caches))(*caches)
+    arr._keep = list(caches)  # the owners of the pools
+    return arr
 
 
 def paged_kv(k_pool, v_pool, page_table, kv_lens, *, n_kv_heads, page_size, head_dim) -> MfPagedKv:

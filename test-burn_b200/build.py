@@ -26,6 +26,9 @@ SOURCES = [
     HERE / "csrc" / "prefill.cu",
     HERE / "csrc" / "prefill_tc.cu",
     HERE / "csrc" / "attention_api.cu",
+    HERE / "csrc" / "chunk_attention.cu",
+    HERE / "csrc" / "mrope_append.cu",
+    HERE / "csrc" / "page_moves.cu",
     HERE / "csrc" / "peer_exchange.cu",
     HERE / "host" / "host_logic.cpp",
     HERE / "host" / "prefix_cache.cpp",

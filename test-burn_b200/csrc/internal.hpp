@@ -236,6 +236,27 @@ struct MfDecodePlan {
 
 namespace mf {
 
+// Makes the context's device the current one for a scope, so that allocations and launches on its stream work
+// whatever device the caller's thread has selected.
+class DeviceScope {
+  public:
+    explicit DeviceScope(int device)
+    {
+        if (cudaGetDevice(&before_) != cudaSuccess) before_ = -1;
+        if (before_ == device) before_ = -1;
+        else cudaSetDevice(device);
+    }
+    ~DeviceScope()
+    {
+        if (before_ >= 0) cudaSetDevice(before_);
+    }
+    DeviceScope(const DeviceScope &) = delete;
+    DeviceScope &operator=(const DeviceScope &) = delete;
+
+  private:
+    int before_ = -1;
+};
+
 mf_status fail(MfContext *ctx, mf_status code, const char *fmt, ...);
 mf_status check_cuda(MfContext *ctx, cudaError_t e, const char *what);
 mf_status check_launch(MfContext *ctx, const char *what);

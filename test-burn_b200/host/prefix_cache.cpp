@@ -13,9 +13,11 @@
 // changes is the payload: with pages a snapshot is a list of page ids whose reference count is
 // raised, a restore hands the ids to the new sequence, and only a page that the new sequence
 // will write into (the last one when the matched prefix ends inside it) has to be copied first.
+#include <algorithm>
 #include <cstring>
 #include <deque>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include <new>
@@ -212,6 +214,118 @@ mf_status mf_prefix_cache_lookup(MfPrefixCache *cache, const uint32_t *prompt, u
     if (st != MF_OK) return st;
     *matched_out = best_len;
     *n_pages_out = n_pages;
+    return MF_OK;
+}
+
+mf_status mf_page_pool_fork(MfPagePool *pool, const uint32_t *ids, uint32_t n_tokens, uint32_t page_size,
+                            uint32_t *out_ids, uint32_t *copy_src, uint32_t *copy_dst)
+{
+    if (!pool || !copy_src || !copy_dst || (n_tokens && (!ids || !out_ids))) return MF_ERR_INPUT_NOT_FOUND;
+    *copy_src = *copy_dst = UINT32_MAX;
+    if (page_size == 0) return MF_ERR_INVALID_OPERATION;
+    const uint32_t full = n_tokens / page_size;
+    const bool partly = n_tokens % page_size != 0;
+    // entries given back behind a window stay given back for the new owner too
+    for (uint32_t i = 0; i < full + (partly ? 1u : 0u); ++i) {
+        if (ids[i] == UINT32_MAX && i < full) continue;
+        if (ids[i] >= pool->refs.size() || pool->refs[ids[i]] == 0) return MF_ERR_INVALID_OPERATION;
+    }
+    if (partly && pool->free_list.empty()) return MF_ERR_OUT_OF_MEMORY;
+    for (uint32_t i = 0; i < full; ++i) {
+        out_ids[i] = ids[i];
+        if (ids[i] != UINT32_MAX) ++pool->refs[ids[i]];
+    }
+    if (partly) {
+        const uint32_t last = ids[full];
+        const mf_status st = mf_page_pool_alloc(pool, 1, &out_ids[full]);
+        if (st != MF_OK) return st;
+        *copy_src = last;
+        *copy_dst = out_ids[full];
+    }
+    return MF_OK;
+}
+
+mf_status mf_page_pool_release_hidden(MfPagePool *pool, uint32_t *ids, uint32_t n, uint32_t kv_len, uint32_t page_size,
+                                      uint32_t window, uint32_t n_sinks, uint32_t *released)
+{
+    if (!pool || !released || (n && !ids)) return MF_ERR_INPUT_NOT_FOUND;
+    *released = 0;
+    if (page_size == 0) return MF_ERR_INVALID_OPERATION;
+    if (window == 0 || kv_len < window) return MF_OK;
+    // keys [n_sinks, first_seen) are hidden from position kv_len and everything behind it
+    const uint64_t first_seen = (uint64_t)kv_len - window + 1;
+    const uint64_t lo = ((uint64_t)n_sinks + page_size - 1) / page_size;
+    const uint64_t hi = first_seen / page_size < n ? first_seen / page_size : n;
+    for (uint64_t i = lo; i < hi; ++i)
+        if (ids[i] != UINT32_MAX && (ids[i] >= pool->refs.size() || pool->refs[ids[i]] == 0)) return MF_ERR_INVALID_OPERATION;
+    for (uint64_t i = lo; i < hi; ++i)
+        if (ids[i] != UINT32_MAX && pool->refs[ids[i]] > 0) {
+            release_pages(pool, &ids[i], 1);
+            ids[i] = UINT32_MAX;
+            ++*released;
+        }
+    return MF_OK;
+}
+
+mf_status mf_page_pool_compact(MfPagePool *pool, uint32_t *src_out, uint32_t *dst_out, uint32_t cap, uint32_t *n_out)
+{
+    if (!pool || !n_out || (cap && (!src_out || !dst_out))) return MF_ERR_INPUT_NOT_FOUND;
+    const uint32_t n_pages = (uint32_t)pool->refs.size(), live = n_pages - (uint32_t)pool->free_list.size();
+    uint32_t moves = 0;
+    for (uint32_t id = live; id < n_pages; ++id) moves += pool->refs[id] > 0;
+    *n_out = moves;
+    if (moves > cap) return MF_ERR_OUT_OF_MEMORY;
+    uint32_t dst = 0, at = 0;
+    for (uint32_t id = live; id < n_pages; ++id) {
+        if (pool->refs[id] == 0) continue;
+        while (pool->refs[dst] > 0) ++dst;  // as many free ids below `live` as live ones above it
+        src_out[at] = id;
+        dst_out[at] = dst;
+        pool->refs[dst] = pool->refs[id];
+        pool->refs[id] = 0;
+        ++at;
+    }
+    // the free ids are now [live, n_pages); the vector keeps its size, low ids are handed out first
+    for (uint32_t i = 0; i < n_pages - live; ++i) pool->free_list[i] = n_pages - 1 - i;
+    return MF_OK;
+}
+
+// Sorted (src, dst) pairs; false when memory ran out.
+static bool sorted_pairs(const uint32_t *src, const uint32_t *dst, uint32_t n, std::vector<std::pair<uint32_t, uint32_t>> &out)
+{
+    try {
+        out.resize(n);
+    } catch (const std::bad_alloc &) {
+        return false;
+    }
+    for (uint32_t i = 0; i < n; ++i) out[i] = {src[i], dst[i]};
+    std::sort(out.begin(), out.end());
+    return true;
+}
+
+static void remap_ids(uint32_t *ids, uint64_t n_ids, const std::vector<std::pair<uint32_t, uint32_t>> &pairs)
+{
+    for (uint64_t i = 0; i < n_ids; ++i) {
+        const auto it = std::lower_bound(pairs.begin(), pairs.end(), std::make_pair(ids[i], 0u));
+        if (it != pairs.end() && it->first == ids[i]) ids[i] = it->second;
+    }
+}
+
+mf_status mf_remap_page_ids(uint32_t *ids, uint64_t n_ids, const uint32_t *src, const uint32_t *dst, uint32_t n)
+{
+    if ((n_ids && !ids) || (n && (!src || !dst))) return MF_ERR_INPUT_NOT_FOUND;
+    std::vector<std::pair<uint32_t, uint32_t>> pairs;
+    if (!sorted_pairs(src, dst, n, pairs)) return MF_ERR_OUT_OF_MEMORY;
+    remap_ids(ids, n_ids, pairs);
+    return MF_OK;
+}
+
+mf_status mf_prefix_cache_remap(MfPrefixCache *cache, const uint32_t *src, const uint32_t *dst, uint32_t n)
+{
+    if (!cache || (n && (!src || !dst))) return MF_ERR_INPUT_NOT_FOUND;
+    std::vector<std::pair<uint32_t, uint32_t>> pairs;
+    if (!sorted_pairs(src, dst, n, pairs)) return MF_ERR_OUT_OF_MEMORY;
+    for (auto &e : cache->entries) remap_ids(e.pages.data(), e.pages.size(), pairs);
     return MF_OK;
 }
 
