@@ -669,6 +669,14 @@ MF_API mf_status mf_chunk_plan_update(MfContext *ctx, MfChunkPlan *plan, const u
                                       const uint32_t *kv_lens_host);
 MF_API void mf_chunk_plan_destroy(MfContext *ctx, MfChunkPlan *plan);
 MF_API uint32_t mf_chunk_plan_tokens(const MfChunkPlan *plan);
+/* The planner alone, on the host: items_out gets 16 uint32 per item (seq, kv head, first token, tokens, position of
+ * the first token (int32), sink pages, first page behind them, pages, tile begin, tile end, slot, first slot, parts,
+ * ticket, 0, 0), cta_begin_out n_ctas + 1 entries; returns the number of items (items_out is filled when it holds
+ * them), 0 for arguments without a meaning. */
+MF_API uint32_t mf_chunk_plan_build_host(const uint32_t *q_lens_host, const uint32_t *kv_lens_host, uint32_t batch,
+                                         uint32_t n_heads, uint32_t n_kv_heads, uint32_t page_size, uint32_t window,
+                                         uint32_t n_sinks, uint32_t n_ctas, uint32_t *items_out, uint32_t item_capacity,
+                                         uint32_t *cta_begin_out);
 /* q and out: f16, 16-byte aligned; element (token t, head h, dim d) at t * stride_t + h * stride_h + d,
  * strides in elements, multiples of 8.  q is rotated already.  scale >= 0. */
 typedef struct MfPagedChunkArgs {

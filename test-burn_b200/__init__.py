@@ -262,6 +262,7 @@ _SIGNATURES = {
     "mf_chunk_plan_update": (C.c_int32, [vp, vp, vp, vp]),
     "mf_chunk_plan_destroy": (None, [vp, vp]),
     "mf_chunk_plan_tokens": (u32, [vp]),
+    "mf_chunk_plan_build_host": (u32, [vp, vp] + [u32] * 7 + [vp, u32, vp]),
     "mf_paged_chunk_attention": (C.c_int32, [vp, vp, C.POINTER(MfPagedKv), C.POINTER(MfPagedChunkArgs)]),
     "mf_paged_mrope_append": (C.c_int32, [vp, C.POINTER(MfPagedKv), C.POINTER(MfMropeAppendArgs)]),
     "mf_paged_kv8_mrope_append": (C.c_int32, [vp, C.POINTER(MfPagedKv8), C.POINTER(MfMropeAppendArgs)]),
@@ -1004,6 +1005,17 @@ def build_decode_plan_host(kv_lens, n_kv_heads: int, max_ctas: int):
     n = lib.mf_decode_plan_build_host(lens.ctypes.data, lens.shape[0], n_kv_heads, max_ctas, items.ctypes.data, cap,
                                       cta_begin.ctypes.data, C.byref(n_ctas))
     return items[:n].copy(), cta_begin[:n_ctas.value + 1].copy()
+
+
+def build_chunk_plan_host(q_lens, kv_lens, *, n_heads, n_kv_heads, page_size, n_ctas, window=0, sinks=0):
+    """Run the ragged batch's planner on the host.  Returns (items [n, 16] uint32, cta_begin [n_ctas + 1])."""
+    ql, kl = np.ascontiguousarray(q_lens, np.uint32), np.ascontiguousarray(kv_lens, np.uint32)
+    begin = np.zeros(n_ctas + 1, np.uint32)
+    args = (ql.ctypes.data, kl.ctypes.data, ql.size, n_heads, n_kv_heads, page_size, window, sinks, n_ctas)
+    n = lib.mf_chunk_plan_build_host(*args, None, 0, begin.ctypes.data)
+    items = np.zeros((n, 16), np.uint32)
+    lib.mf_chunk_plan_build_host(*args, items.ctypes.data, n, begin.ctypes.data)
+    return items, begin
 
 
 def build_decode_plan_host_clusters(kv_lens, n_kv_heads: int, max_ctas: int, max_cluster: int = 16, clusters_of_16: int = 0,

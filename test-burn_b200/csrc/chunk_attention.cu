@@ -1,26 +1,63 @@
-// Attention of a ragged batch of new tokens over a paged cache: causal, optionally with a sliding window and
-// first tokens that stay visible (sinks).
+// Attention of a ragged batch of new tokens over a paged cache on the tcgen05 tensor cores: causal, optionally with a
+// sliding window and first tokens that stay visible (sinks).
 //
 //   out[t, h] = sum_k w_k V[k] / sum_k w_k,   w_k = exp(scale * q[t, h] . K[k] - max_k),   k visible to t
 //
-// One warp per (token, query head) walks the visible keys with a running maximum and sum (f32), every lane
-// holding D / 32 dims of q and of the accumulator.
+// One persistent CTA per SM walks its items of the plan (chunk_plan.hpp).  The rows of a unit are (token, query head of
+// the kv head) pairs, so that one pass over a kv head's keys serves all its query heads, and the causal diagonal and
+// the window's edge are 128 / G tokens wide instead of 128.
+//
+// Two streams, each a 128-row score tile S_s and an output tile O_s in TMEM with a softmax group of its own:
+//   more than 128 rows   the streams are the two query tiles, both work on every key tile ("paired rows")
+//   up to 128 rows       both streams hold the same rows, stream s takes the key tiles s, s + 2, ... and the two states
+//                        are merged when the item ends ("paired keys"): decode and short chunks
+// A stream is one chain  S = Q K^T -> max, exp, P (f16, over S) -> O += P V -> next tile;  while its softmax group
+// works, the tensor pipe works for the other stream.  Nothing is handed from one group to the other between tiles.
+//
+//   warps 0-3, 4-7  softmax groups (one thread per row = TMEM lane)   warp 8   TMA producer, one copy per page and tile
+//   warps 9, 10     issue the products of streams 0, 1                warp 11  loads q, allocates TMEM
+//
+// K and V tiles share one ring in the order in which the products want them.  A (page, kv head) run lands as
+// [8-row group][half][8 rows][128 bytes], so the 128 rows of a tile are evenly spaced 8-row groups whatever the page
+// size, and both operands (K by rows, V by columns) take one descriptor per tile.
+//
+// O is rescaled only when a row's maximum has grown by more than 2^8 since the last rescale; weights are then at most
+// 256 and are rounded to f16 for the product (2^-11 of each), sums, maxima and accumulators are f32.
+//
+// Rows of a tile that no row of the unit sees (the end of the cache, the edge of the window) are cleared in V: their
+// weight is zero, but zero times a stale NaN is not.  A value row that some rows see and others do not can only hurt the
+// others when it is not finite; then the output is not finite either, and such a row is walked again key by key
+// (walk_row).
+//
+// TMEM columns (512): S_0/P_0 [0,128)  S_1/P_1 [128,256)  O_0 [256,384)  O_1 [384,512).
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <cstring>
 #include <new>
 #include <vector>
 
+#include "chunk_plan.hpp"
 #include "internal.hpp"
 #include "ptx.cuh"
+#include "tcgen05.cuh"
 
 struct MfChunkPlan {
     uint32_t batch = 0, n_heads = 0, n_kv_heads = 0, head_dim = 0, page_size = 0, window = 0, n_sinks = 0;
     uint32_t max_tokens = 0, tokens = 0, max_pages = 0;
+    uint32_t n_ctas = 0, begin_words = 0;  // cta_begin, padded to whole items
+    uint64_t item_capacity = 0;
     int device = 0;
-    uint32_t *d_meta = nullptr;  // [batch + 1] q_begin, [batch] kv_lens
+    std::vector<mf::ChunkItem> h_items;
+    std::vector<uint32_t> h_begin;
+    // [begin_words] cta_begin, [item_capacity] items; two pinned copies used in turn, each guarded by the event
+    // recorded after its upload
+    uint32_t *d_list = nullptr;
     uint32_t *pinned[2] = {nullptr, nullptr};
     cudaEvent_t staged[2] = {nullptr, nullptr};
     uint32_t next_stage = 0;
+    float *d_acc = nullptr, *d_ml = nullptr;  // partial results: [slot][256 rows][D], [slot][256 rows][2]
+    uint32_t *d_tickets = nullptr;
 };
 
 namespace mf {
@@ -28,72 +65,585 @@ namespace {
 
 constexpr uint32_t kMaxGroup = 64;
 constexpr uint32_t kMaxLen = 1u << 30;  // positions and tile arithmetic stay inside 32 bits
+constexpr uint32_t kTile = kChunkTile;
+constexpr uint32_t kThreads = 384;
+constexpr uint32_t kProducerWarp = 8, kIssuerWarp = 9, kQWarp = 11;
+constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr float kNegInf = -1e30f;
+constexpr float kRescaleThreshold = 8.0f;  // log2 of the largest weight kept in P
+constexpr uint32_t kHalfTile = kTile * 128;
+
+__host__ __device__ constexpr uint32_t tile_bytes(uint32_t d) { return kTile * d * 2; }
+__host__ __device__ constexpr uint32_t ring_slots(uint32_t d) { return d == 128 ? 5 : 10; }
+enum Bar : uint32_t {
+    kSFull = 0,   // [2] scores of the stream's next tile are in S (and its last P V has completed)
+    kPFull = 2,   // [2] weights are in P, O has been rescaled if needed
+    kOFull = 4,   // [2] the item's last P V has completed
+    kOFree = 6,   // [2] the item's O has been read (8 arrivals)
+    kQFull = 8,
+    kQFree = 9,   // 2 arrivals: the streams' last Q K^T of the item
+    kFull = 10    // [slots], then empty [slots] (2 arrivals: the streams)
+};
+__host__ __device__ constexpr uint32_t num_bars(uint32_t d) { return kFull + 2 * ring_slots(d); }
+constexpr uint32_t kMlBytes = 2 * kTile * 8;  // (m, l) of the two streams' rows
+__host__ __device__ constexpr uint32_t smem_bytes(uint32_t d)
+{
+    return tile_bytes(d) * (2 + ring_slots(d)) + kMlBytes + num_bars(d) * 8 + 16;
+}
+static_assert(smem_bytes(128) <= 227 * 1024 && smem_bytes(64) <= 227 * 1024, "shared memory");
 
 struct ChunkParams {
     const __half *q;
     __half *out;
-    const __half *k_pool, *v_pool;
-    const uint32_t *page_table, *q_begin, *kv_lens;
-    uint32_t *status;
+    const __half *k_pool, *v_pool;  // walk_row only
+    const uint32_t *page_table;
+    const uint32_t *list;  // cta_begin, then the items
+    float *acc, *ml;
+    uint32_t *tickets, *status;
     uint64_t q_stride_t, q_stride_h, out_stride_t, out_stride_h;
-    uint32_t batch, n_heads, n_kv_heads, group, page_size, pt_stride, n_pages, window, n_sinks;
+    uint32_t begin_words, n_kv_heads, group, page_shift, pt_stride, n_pages, window, n_sinks;
     float scale_log2;
 };
 
-template <uint32_t D>
-__global__ void __launch_bounds__(256) chunk_rows_kernel(const ChunkParams p)
+__device__ __forceinline__ ChunkItem load_item(const ChunkParams &p, uint32_t i)
 {
-    constexpr uint32_t E = D / 32;  // dims per lane: [lane * E, lane * E + E)
-    const uint32_t lane = threadIdx.x & 31;
-    const uint64_t wid = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-    const uint32_t h = (uint32_t)(wid % p.n_heads);
-    const uint64_t t = wid / p.n_heads;
-    if (t >= p.q_begin[p.batch]) return;
-    uint32_t lo = 0, hi = p.batch;  // the sequence whose tokens hold t
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (p.q_begin[mid] <= t) lo = mid;
-        else hi = mid;
-    }
-    const uint32_t b = lo, kvh = h / p.group;
-    const int64_t pos = (int64_t)p.kv_lens[b] - (p.q_begin[b + 1] - t);
-    float q[E], acc[E];
-    const __half *qp = p.q + t * p.q_stride_t + h * p.q_stride_h + lane * E;
+    ChunkItem it;
+    const uint4 *src = reinterpret_cast<const uint4 *>(p.list + p.begin_words) + (size_t)i * 4;
+    uint4 *dst = reinterpret_cast<uint4 *>(&it);
 #pragma unroll
-    for (uint32_t e = 0; e < E; ++e) {
-        q[e] = __half2float(qp[e]);
-        acc[e] = 0.f;
-    }
-    float m = -1e30f, l = 0.f;
-    const uint32_t *table = p.page_table + (size_t)b * p.pt_stride;
-    auto walk = [&](int64_t k0, int64_t k1) {
-        for (int64_t k = k0; k < k1; ++k) {
-            const uint32_t page = table[k / p.page_size];
-            if (page >= p.n_pages) {
-                if (lane == 0) atomicOr(p.status, kStatusBadPage);
-                continue;
-            }
-            const size_t row = (((size_t)page * p.n_kv_heads + kvh) * p.page_size + k % p.page_size) * D + lane * E;
+    for (uint32_t j = 0; j < 4; ++j) dst[j] = __ldg(src + j);
+    return it;
+}
+
+// What a row at position pos sees, in columns of the unit's page list: [0, a) and [b, c).
+struct Visible {
+    int32_t a, b, c;
+};
+__device__ __forceinline__ Visible visible(const ChunkParams &p, const ChunkItem &it, int32_t pos)
+{
+    Visible v{0, 0, 0};
+    if (pos < 0) return v;
+    const int32_t lo = p.window && (uint32_t)pos >= p.window ? pos - (int32_t)p.window + 1 : 0;
+    const int32_t shift = ((int32_t)it.first_page - (int32_t)it.n_sink_pages) << p.page_shift;
+    v.a = min((int32_t)min(p.n_sinks, 0x7FFFFFFFu), lo);
+    v.b = lo - shift;
+    v.c = pos + 1 - shift;
+    if (v.a >= v.b) v.a = v.b = 0;  // the sinks reach the window: one range
+    return v;
+}
+__device__ __forceinline__ uint32_t page_entry(const ChunkItem &it, uint32_t v)
+{
+    return v < it.n_sink_pages ? v : v - it.n_sink_pages + it.first_page;
+}
+__device__ __forceinline__ uint32_t low_bits(int32_t n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
+
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// sum_x 2^(s_x - m) V[x][d0 .. d0 + dims) over the columns of the item that the row sees, key by key; one warp, result
+// in lanes * dims / 32 consecutive dims.  Rare: only for rows whose product with the whole tile was not finite.
+template <uint32_t D>
+__device__ __noinline__ void walk_row(const ChunkParams &p, const ChunkItem &it, const __half *q, int32_t pos, float m, uint32_t d0,
+                                      uint32_t dims, float (&acc)[D / 32])
+{
+    const uint32_t lane = threadIdx.x & 31, E = dims / 32, P = 1u << p.page_shift;
+    const Visible vis = visible(p, it, pos);
+#pragma unroll
+    for (uint32_t e = 0; e < D / 32; ++e) acc[e] = 0.f;
+    const int32_t x0 = it.tile_begin * kTile, x1 = it.tile_end * kTile;
+    for (uint32_t part = 0; part < 2; ++part) {
+        const int32_t lo = max(x0, part ? vis.b : 0), hi = min(x1, part ? vis.c : vis.a);
+        for (int32_t x = lo; x < hi; ++x) {
+            const uint32_t entry = page_entry(it, (uint32_t)x >> p.page_shift);
+            const uint32_t page = entry < p.pt_stride ? p.page_table[(size_t)it.seq * p.pt_stride + entry] : 0xFFFFFFFFu;
+            if (page >= p.n_pages) continue;
+            const size_t row = ((((size_t)page * p.n_kv_heads + it.kvh) << p.page_shift) + ((uint32_t)x & (P - 1))) * D;
             float s = 0.f;
-#pragma unroll
-            for (uint32_t e = 0; e < E; ++e) s = fmaf(q[e], __half2float(p.k_pool[row + e]), s);
+            for (uint32_t d = lane; d < D; d += 32) s = fmaf(__half2float(q[d]), __half2float(p.k_pool[row + d]), s);
 #pragma unroll
             for (uint32_t o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            s *= p.scale_log2;
-            const float m_new = fmaxf(m, s), a = exp2f(m - m_new), w = exp2f(s - m_new);
-            l = l * a + w;
-#pragma unroll
-            for (uint32_t e = 0; e < E; ++e) acc[e] = fmaf(w, __half2float(p.v_pool[row + e]), acc[e] * a);
-            m = m_new;
+            const float w = fast_exp2(fmaf(s, p.scale_log2, -m));
+            for (uint32_t e = 0; e < E; ++e) acc[e] = fmaf(w, __half2float(p.v_pool[row + d0 + lane * E + e]), acc[e]);
+        }
+    }
+}
+
+// Rows [dead0, dead1) of a V tile are cleared by one softmax group (128 threads).
+template <uint32_t D>
+__device__ __noinline__ void clear_rows(uint8_t *v_tile, int32_t dead0, int32_t dead1, uint32_t gtid)
+{
+    constexpr uint32_t C = D / 8;  // 16-byte units per row
+    for (uint32_t i = gtid; i < (uint32_t)max(dead1 - dead0, 0) * C; i += 128) {
+        const uint32_t r = dead0 + i / C, c = i % C;
+        *reinterpret_cast<uint4 *>(v_tile + (r >> 3) * (16 * D) + (c >> 3) * 1024 + (r & 7) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+    }
+    fence_proxy_async();
+}
+
+template <uint32_t D>
+__global__ void __launch_bounds__(kThreads, 1)
+chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ ChunkParams p)
+{
+    constexpr uint32_t kBytes = tile_bytes(D), kSlots = ring_slots(D);
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t q_smem = smem_u32(smem), ring = q_smem + 2 * kBytes;
+    float2 *ml_s = reinterpret_cast<float2 *>(smem + kBytes * (2 + kSlots));  // [stream][row]
+    const uint32_t bars = q_smem + kBytes * (2 + kSlots) + kMlBytes;
+    volatile uint32_t *words = reinterpret_cast<volatile uint32_t *>(smem + kBytes * (2 + kSlots) + kMlBytes + num_bars(D) * 8);
+    volatile uint32_t *abort_flag = words + 1;
+    auto bar = [&](uint32_t i) { return bars + i * 8; };
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t G = p.group, half_tok = kTile / G;
+    const uint32_t item0 = __ldg(p.list + blockIdx.x), item1 = __ldg(p.list + blockIdx.x + 1);
+    if (item0 >= item1) return;
+    if (q_smem & 1023u) {  // the swizzled tiles need it; dynamic shared memory starts there when nothing is static
+        if (tid == 0) atomicOr(p.status, 1u);
+        return;
+    }
+    if (tid == 0) {
+        for (uint32_t s = 0; s < 2; ++s) {
+            mbar_init(bar(kSFull + s), 1);
+            mbar_init(bar(kPFull + s), 4);
+            mbar_init(bar(kOFull + s), 1);
+            mbar_init(bar(kOFree + s), 8);
+        }
+        mbar_init(bar(kQFull), 1);
+        mbar_init(bar(kQFree), 2);
+        for (uint32_t s = 0; s < kSlots; ++s) {
+            mbar_init(bar(kFull + s), 1);
+            mbar_init(bar(kFull + kSlots + s), 2);
+        }
+        *abort_flag = 0;
+        mbar_fence_init();
+        fence_proxy_async();
+    }
+    if (warp == kQWarp) {
+        tmem_alloc(smem_u32(const_cast<uint32_t *>(words)), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *words;
+
+    auto wait = [&](uint32_t b, uint32_t parity, uint32_t code) {
+        if (mbar_try_wait(b, parity)) return;
+        if (!*abort_flag && !mbar_wait_bounded(b, parity, kWaitNs)) {
+            *abort_flag = 1;
+            atomicOr(p.status, code);
         }
     };
-    const int64_t first = p.window ? (pos - (int64_t)p.window + 1 > 0 ? pos - (int64_t)p.window + 1 : 0) : 0;
-    walk(0, min((int64_t)p.n_sinks, first));
-    walk(first, pos + 1);
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    __half *op = p.out + t * p.out_stride_t + h * p.out_stride_h + lane * E;
+
+    if (warp == kProducerWarp) {
+        // ------------------------------------------------------------------ K/V producer (whole warp) ---
+        const uint32_t per_tile = kTile >> p.page_shift, page_bytes = D * 2u << p.page_shift;
+        const uint32_t none = p.n_pages * p.n_kv_heads;  // coordinate behind the pool: arrives as zeros
+        uint32_t slot = 0, phase = 0;
+        auto read_id = [&](const ChunkItem &it, uint32_t t) -> uint32_t {
+            const uint32_t v = t * per_tile + lane;
+            if (lane >= per_tile || v >= it.n_pages) return 0u;
+            // (a replayed launch can meet a plan whose sequences have outgrown the captured table)
+            const uint32_t entry = page_entry(it, v);
+            return entry < p.pt_stride ? __ldg(p.page_table + (size_t)it.seq * p.pt_stride + entry) : 0xFFFFFFFFu;
+        };
+        auto load = [&](const CUtensorMap *tm, const ChunkItem &it, uint32_t t, uint32_t id) {
+            const uint32_t n = min(per_tile, it.n_pages - t * per_tile);
+            if (lane == 0) {
+                wait(bar(kFull + kSlots + slot), phase ^ 1, 2u);
+                mbar_arrive_expect_tx(bar(kFull + slot), n * page_bytes);
+            }
+            __syncwarp();
+            if (lane < n) {
+                if (id >= p.n_pages) atomicOr(p.status, kStatusBadPage);
+                tma_load_5d_last(ring + slot * kBytes + lane * page_bytes, tm, (int32_t)(id < p.n_pages ? id * p.n_kv_heads + it.kvh : none),
+                                 bar(kFull + slot));
+            }
+            if (++slot == kSlots) slot = 0, phase ^= 1;
+        };
+        if (lane == 0) {
+            tma_prefetch_desc(&tm_k);
+            tma_prefetch_desc(&tm_v);
+        }
+        ChunkItem it = load_item(p, item0);
+        uint32_t id0 = read_id(it, it.tile_begin), id1 = read_id(it, it.tile_begin + 1);
+        for (uint32_t i = item0; i < item1; ++i) {
+            const ChunkItem next = i + 1 < item1 ? load_item(p, i + 1) : it;
+            const uint32_t step = it.n_tok > half_tok ? 1 : 2;
+            for (uint32_t t = it.tile_begin; t < it.tile_end; t += step) {
+                // page ids of the following tiles are requested before this one's copies wait for their slots
+                const bool last = t + step >= it.tile_end;
+                const uint32_t n0 = last ? read_id(next, next.tile_begin) : read_id(it, t + step);
+                const uint32_t n1 = last ? read_id(next, next.tile_begin + 1) : read_id(it, t + step + 1);
+                const bool two = step == 2 && t + 1 < it.tile_end;
+                load(&tm_k, it, t, id0);
+                if (two) load(&tm_k, it, t + 1, id1);
+                load(&tm_v, it, t, id0);
+                if (two) load(&tm_v, it, t + 1, id1);
+                id0 = n0;
+                id1 = n1;
+            }
+            if (it.tile_begin == it.tile_end) {
+                id0 = read_id(next, next.tile_begin);
+                id1 = read_id(next, next.tile_begin + 1);
+            }
+            it = next;
+        }
+        // Nothing may still be on its way into this CTA's shared memory when it ends (it is not, unless a wait ran out).
+        if (lane == 0 && *abort_flag)
+            for (uint32_t s = 0; s < kSlots; ++s) mbar_wait_bounded(bar(kFull + s), s < slot ? phase : phase ^ 1, kWaitNs / 16);
+    } else if (warp == kQWarp) {
+        // ------------------------------------------------------------------------- q (whole warp) ---
+        uint32_t used = 0;
+        for (uint32_t i = item0; i < item1; ++i) {
+            const ChunkItem it = load_item(p, i);
+            if (it.tile_begin == it.tile_end) continue;
+            if (used) wait(bar(kQFree), (used - 1) & 1, 4u);
+            ++used;
+            constexpr uint32_t C = D / 8;
+            const uint32_t rows = it.n_tok * G, per_stream = half_tok * G;
+            for (uint32_t x = lane; x < rows * C; x += 32) {
+                uint32_t r = x / C;
+                const uint32_t c = x % C, tok = r / G, g = r - tok * G;
+                uint32_t dst = q_smem;
+                if (r >= per_stream) r -= per_stream, dst += kBytes;
+                cp_async16(dst + (c >> 3) * kHalfTile + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+                           p.q + (it.tok0 + (uint64_t)tok) * p.q_stride_t + (uint64_t)(it.kvh * G + g) * p.q_stride_h + c * 8);
+            }
+            cp_async16_wait_all();
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(kQFull));
+        }
+    } else if (warp >= kIssuerWarp) {
+        // ------------------------------------------------------------------ products of one stream ---
+        if (lane == 0) {
+            const uint32_t s = warp - kIssuerWarp;
+            constexpr uint32_t kIdescQK = instr_desc_f16(kTile, kTile, 0), kIdescPV = instr_desc_f16(kTile, D, 1);
+            constexpr uint32_t kGroupStride = 16 * D;  // bytes between 8-row groups of a K or V tile
+            const uint32_t s_tm = tmem + s * 128, o_tm = tmem + 256 + s * 128;
+            uint32_t slot = 0, phase = 0, q_phase = 0, p_phase = 0, o_uses = 0;
+            auto next_slot = [&]() {
+                if (++slot == kSlots) slot = 0, phase ^= 1;
+            };
+            auto skip = [&]() {  // a tile of the other stream
+                wait(bar(kFull + slot), phase, 8u);
+                mbar_arrive(bar(kFull + kSlots + slot));
+                next_slot();
+            };
+            for (uint32_t i = item0; i < item1; ++i) {
+                const ChunkItem it = load_item(p, i);
+                const uint32_t n = it.tile_end - it.tile_begin;
+                if (n == 0) continue;
+                const bool paired_rows = it.n_tok > half_tok;
+                const uint32_t step = paired_rows ? 1 : 2, mine = paired_rows ? n : (n + 1 - s) / 2;
+                const uint64_t q_desc = smem_desc(q_smem + (paired_rows ? s * kBytes : 0), 16, 1024);
+                wait(bar(kQFull), q_phase, 16u);
+                q_phase ^= 1;
+                if (mine == 0) mbar_arrive(bar(kQFree));
+                for (uint32_t j = 0, t = 0; t < n; ++j, t += step) {
+                    const bool two = step == 2 && t + 1 < n, own = paired_rows || s == 0 || two;
+                    if (step == 2 && s == 1) skip();
+                    if (own) {
+                        wait(bar(kFull + slot), phase, 16u);
+                        tc_fence_after();
+                        const uint64_t k_desc = smem_desc(ring + slot * kBytes, 16, kGroupStride);
 #pragma unroll
-    for (uint32_t e = 0; e < E; ++e) op[e] = __float2half_rn(acc[e] * inv);
+                        for (uint32_t kk = 0; kk < D / 16; ++kk)
+                            tc_mma_ss(s_tm, q_desc + (((kk >> 2) * kHalfTile + (kk & 3) * 32) >> 4),
+                                      k_desc + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4), kIdescQK, kk > 0);
+                        tc_commit(bar(kSFull + s));
+                        tc_commit(bar(kFull + kSlots + slot));
+                        if (j + 1 == mine) tc_commit(bar(kQFree));
+                        next_slot();
+                    }
+                    if (two && s == 0) skip();
+                    if (step == 2 && s == 1) skip();
+                    if (own) {
+                        wait(bar(kFull + slot), phase, 32u);
+                        wait(bar(kPFull + s), p_phase, 64u);
+                        p_phase ^= 1;
+                        if (j == 0 && o_uses) wait(bar(kOFree + s), (o_uses - 1) & 1, 128u);
+                        tc_fence_after();
+                        const uint64_t v_desc = smem_desc(ring + slot * kBytes, 1024, kGroupStride);
+#pragma unroll
+                        for (uint32_t kk = 0; kk < kTile / 16; ++kk)
+                            tc_mma_ts(o_tm, s_tm + kk * 8, v_desc + ((kk * 2 * kGroupStride) >> 4), kIdescPV, (j > 0 || kk > 0) ? 1u : 0u);
+                        tc_commit(bar(kFull + kSlots + slot));
+                        if (j + 1 == mine) tc_commit(bar(kOFull + s));
+                        next_slot();
+                    }
+                    if (two && s == 0) skip();
+                }
+                if (mine) ++o_uses;
+            }
+            // The products have to be over before the TMEM goes back (they are, unless a wait ran out).
+            if (o_uses) wait(bar(kOFull + s), (o_uses - 1) & 1, 256u);
+        }
+        __syncwarp();
+    } else {
+        // -------------------------------------------------------------- softmax groups / epilogue ---
+        const uint32_t s = warp >> 2, quad = warp & 3, r_in = quad * 32 + lane, gtid = tid & 127;
+        const uint32_t lane_base = (quad * 32u) << 16;
+        const uint32_t s_tm = tmem + lane_base + s * 128, o_base = tmem + lane_base + 256;
+        uint32_t s_phase = 0, o_uses[2] = {0, 0}, loads = 0;  // loads: tiles the ring has seen before this item
+        for (uint32_t i = item0; i < item1; ++i) {
+            const ChunkItem it = load_item(p, i);
+            const uint32_t n = it.tile_end - it.tile_begin;
+            const bool paired_rows = it.n_tok > half_tok;
+            const uint32_t tok_first = paired_rows ? s * half_tok : 0;
+            const uint32_t rows = min(half_tok, it.n_tok - tok_first) * G;
+            const bool valid = r_in < rows, busy = quad * 32 < rows;  // busy: the warp has rows
+            const uint32_t tok = tok_first + (valid ? r_in / G : 0), head = it.kvh * G + (valid ? r_in % G : 0);
+            const int32_t pos = it.pos0 + (int32_t)tok;
+            const Visible vis = visible(p, it, pos);
+            // columns that some row of the unit sees: [0, any_a), [any_b, any_c)
+            const Visible v_first = visible(p, it, max(it.pos0, 0)), v_last = visible(p, it, it.pos0 + (int32_t)it.n_tok - 1);
+            const uint32_t mine = paired_rows ? n : (n + 1 - s) / 2;
+            float m_ref = kNegInf, l = 0.f;
+            for (uint32_t j = 0; j < mine; ++j) {
+                const uint32_t t = paired_rows ? j : 2 * j + s;
+                const int32_t x0 = (int32_t)((it.tile_begin + t) * kTile);
+                wait(bar(kSFull + s), s_phase, 512u);
+                s_phase ^= 1;
+                tc_fence_after();
+                if (busy) {
+                    const bool whole = __all_sync(0xffffffffu, !valid || (vis.b <= x0 && vis.c >= x0 + (int32_t)kTile) || vis.a >= x0 + (int32_t)kTile);
+                    uint32_t r[kTile];
+                    auto fetch = [&]() {
+#pragma unroll
+                        for (uint32_t c = 0; c < kTile / 32; ++c) tmem_ld32(s_tm + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
+                        tc_wait_ld();
+                        if (!whole) {
+#pragma unroll
+                            for (uint32_t c = 0; c < kTile / 32; ++c) {
+                                const int32_t xc = x0 + (int32_t)c * 32;
+                                const uint32_t see = low_bits(vis.a - xc) | (low_bits(vis.c - xc) & ~low_bits(vis.b - xc));
+#pragma unroll
+                                for (uint32_t q = 0; q < 32; ++q)
+                                    if (!((see >> q) & 1u)) r[c * 32 + q] = 0xFF800000u;  // -inf: weight exactly 0
+                            }
+                        }
+                    };
+                    fetch();
+                    float mx0 = -3.0e38f, mx1 = -3.0e38f, mx2 = -3.0e38f, mx3 = -3.0e38f;
+#pragma unroll
+                    for (uint32_t q = 0; q < kTile; q += 8) {
+                        mx0 = max3(mx0, __uint_as_float(r[q]), __uint_as_float(r[q + 1]));
+                        mx1 = max3(mx1, __uint_as_float(r[q + 2]), __uint_as_float(r[q + 3]));
+                        mx2 = max3(mx2, __uint_as_float(r[q + 4]), __uint_as_float(r[q + 5]));
+                        mx3 = max3(mx3, __uint_as_float(r[q + 6]), __uint_as_float(r[q + 7]));
+                    }
+                    const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
+                    const float m_new = mx > -3.0e38f ? mx * p.scale_log2 : kNegInf;
+                    const bool grow = valid && m_new > m_ref + kRescaleThreshold;
+                    const float m_old = m_ref;
+                    if (grow) m_ref = m_new;
+                    if (j > 0 && __any_sync(0xffffffffu, grow)) {
+                        const float alpha = fast_exp2(m_old - m_ref);
+                        l *= alpha;
+#pragma unroll 1
+                        for (uint32_t c = 0; c < D / 32; ++c) {
+                            uint32_t ob[32];
+                            tmem_ld32(o_base + s * 128 + c * 32, ob);
+                            tc_wait_ld();
+#pragma unroll
+                            for (uint32_t q = 0; q < 32; ++q) ob[q] = __float_as_uint(__uint_as_float(ob[q]) * alpha);
+                            tmem_st32(o_base + s * 128 + c * 32, ob);
+                        }
+                        tc_wait_st();
+                        fetch();  // rather than keeping the scores in registers across this rare block
+                    }
+                    const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(-m_ref, -m_ref);
+                    float2 acc_a = make_float2(0.f, 0.f), acc_b = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (uint32_t c = 0; c < kTile / 32; ++c) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (uint32_t q = 0; q < 16; ++q) {
+                            const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c * 32 + 2 * q]), __uint_as_float(r[c * 32 + 2 * q + 1])), sc2, nm2);
+                            float2 w;
+                            w.x = fast_exp2(x.x);
+                            w.y = fast_exp2(x.y);
+                            if (q & 1) acc_b = __fadd2_rn(acc_b, w);
+                            else acc_a = __fadd2_rn(acc_a, w);
+                            pk[q] = pack_f16x2(w.x, w.y);
+                        }
+                        tmem_st16(s_tm + c * 16, pk);
+                    }
+                    const float2 acc = __fadd2_rn(acc_a, acc_b);
+                    l += acc.x + acc.y;
+                }
+                // Dead rows of this tile, relative to it: [any_a, any_b) and [any_c, end).
+                const int32_t end = (int32_t)kTile, gap0 = max(v_last.a - x0, 0), gap1 = min(v_first.b - x0, end);
+                const int32_t tail = v_last.c - x0;
+                if (gap0 < gap1 || tail < end) {
+                    uint32_t load = loads + (paired_rows ? 2 * j + 1 : 4 * j + ((2 * j + 1 < n) ? 2 + s : 1));
+                    const uint32_t slot = load % kSlots;
+                    wait(bar(kFull + slot), (load / kSlots) & 1, 1024u);
+                    uint8_t *v_tile = smem + 2 * kBytes + slot * kBytes;
+                    clear_rows<D>(v_tile, gap0, gap1, gtid);
+                    clear_rows<D>(v_tile, max(tail, 0), end, gtid);
+                }
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(kPFull + s));
+            }
+            loads += 2 * n;
+
+            // ---- the item's rows ------------------------------------------------------------------------
+            // paired rows: group s has all D dims of its own rows; paired keys: dims [s * D/2, (s + 1) * D/2) of the
+            // same rows, from both streams' states.
+            const bool act0 = n > 0 && (paired_rows ? s == 0 : true), act1 = n > 0 && (paired_rows ? s == 1 : n > 1);
+            float f0 = 1.f, f1 = 0.f;  // factors of O_own / (O_0, O_1)
+            if (!paired_rows) {
+                ml_s[s * kTile + r_in] = make_float2(m_ref, l);
+                if (mine) wait(bar(kOFull + s), o_uses[s] & 1, 2048u);
+                named_bar_sync(9, 256);
+                const float2 x0 = ml_s[r_in], x1 = ml_s[kTile + r_in];
+                named_bar_sync(10, 256);  // the next item may publish
+                m_ref = fmaxf(x0.x, x1.x);
+                f0 = fast_exp2(x0.x - m_ref);
+                f1 = fast_exp2(x1.x - m_ref);
+                l = x0.y * f0 + x1.y * f1;
+            } else if (n) {
+                wait(bar(kOFull + s), o_uses[s] & 1, 2048u);
+            }
+            tc_fence_after();
+            const bool cut = it.n_parts > 1;
+            const float norm = cut ? 1.f : (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));  // a sum that is not a number shows
+            f0 *= norm;
+            f1 *= norm;
+            const uint32_t d0 = paired_rows ? 0 : s * (D / 2), dims = paired_rows ? D : D / 2;
+            const uint32_t slot_row = (paired_rows ? s * kTile : 0) + r_in;
+            float *part = p.acc + ((size_t)it.slot * 2 * kTile + slot_row) * D + d0;
+            __half *dst = p.out + (it.tok0 + (uint64_t)tok) * p.out_stride_t + (uint64_t)head * p.out_stride_h + d0;
+            bool odd = false;  // a value that is not finite although the sum of the weights is
+            if (busy) {
+#pragma unroll 1
+                for (uint32_t c = 0; c < dims / 32; ++c) {
+                    float o[32];
+#pragma unroll
+                    for (uint32_t q = 0; q < 32; ++q) o[q] = 0.f;
+                    if (n) {
+                        tmem_ld32(o_base + (paired_rows ? s * 128 : 0) + d0 + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
+                        tc_wait_ld();
+#pragma unroll
+                        for (uint32_t q = 0; q < 32; ++q) o[q] = f0 == 0.f ? 0.f : o[q] * f0;
+                        if (!paired_rows && n > 1) {
+                            uint32_t o1[32];
+                            tmem_ld32(o_base + 128 + d0 + c * 32, o1);
+                            tc_wait_ld();
+#pragma unroll
+                            for (uint32_t q = 0; q < 32; ++q) o[q] += f1 == 0.f ? 0.f : __uint_as_float(o1[q]) * f1;
+                        }
+                    }
+                    if (valid) {
+#pragma unroll
+                        for (uint32_t q = 0; q < 32; ++q) odd |= !(fabsf(o[q]) <= 3.0e38f);
+                        if (cut) {
+#pragma unroll
+                            for (uint32_t q = 0; q < 32; q += 4)
+                                __stcg(reinterpret_cast<float4 *>(part + c * 32 + q), make_float4(o[q], o[q + 1], o[q + 2], o[q + 3]));
+                        } else {
+#pragma unroll
+                            for (uint32_t q = 0; q < 32; q += 8)
+                                *reinterpret_cast<uint4 *>(dst + c * 32 + q) =
+                                    make_uint4(pack_f16x2(o[q], o[q + 1]), pack_f16x2(o[q + 2], o[q + 3]), pack_f16x2(o[q + 4], o[q + 5]),
+                                               pack_f16x2(o[q + 6], o[q + 7]));
+                        }
+                    }
+                }
+            }
+            // O has been read: the next item's first product may overwrite it.
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0 && n) {
+                if (paired_rows) {
+                    mbar_arrive_n(bar(kOFree + s), 2);
+                } else {
+                    mbar_arrive(bar(kOFree));
+                    if (n > 1) mbar_arrive(bar(kOFree + 1));
+                }
+            }
+            if (act0 || (paired_rows && n)) ++o_uses[0];
+            if (act1 || (paired_rows && n)) ++o_uses[1];
+            uint32_t again = __ballot_sync(0xffffffffu, odd && fabsf(l) <= 3.0e38f && fabsf(m_ref) <= 3.0e38f);
+            while (again) {
+                const uint32_t src = __ffs(again) - 1;
+                again &= again - 1;
+                const uint32_t w_tok = __shfl_sync(0xffffffffu, tok, src), w_head = __shfl_sync(0xffffffffu, head, src);
+                const float w_m = __shfl_sync(0xffffffffu, m_ref, src), w_norm = __shfl_sync(0xffffffffu, norm, src);
+                float acc[D / 32];
+                walk_row<D>(p, it, p.q + (it.tok0 + (uint64_t)w_tok) * p.q_stride_t + (uint64_t)w_head * p.q_stride_h, it.pos0 + (int32_t)w_tok,
+                            w_m, d0, dims, acc);
+                const uint32_t E = dims / 32;
+                for (uint32_t e = 0; e < E; ++e) {
+                    const uint32_t d = lane * E + e;
+                    if (cut)
+                        __stcg(p.acc + ((size_t)it.slot * 2 * kTile + (paired_rows ? s * kTile : 0) + quad * 32 + src) * D + d0 + d, acc[e]);
+                    else
+                        p.out[(it.tok0 + (uint64_t)w_tok) * p.out_stride_t + (uint64_t)w_head * p.out_stride_h + d0 + d] = __float2half_rn(acc[e] * w_norm);
+                }
+                __syncwarp();
+            }
+            if (cut) {
+                if (valid && (paired_rows || s == 0))
+                    __stcg(reinterpret_cast<float2 *>(p.ml) + (size_t)it.slot * 2 * kTile + slot_row, make_float2(m_ref, l));
+                __threadfence();
+                named_bar_sync(9, 256);
+                if (tid == 0) {
+                    const uint32_t done = atomicAdd(p.tickets + it.counter, 1u) + 1;
+                    words[2] = done == it.n_parts;
+                    if (done == it.n_parts) p.tickets[it.counter] = 0;  // for the next launch
+                }
+                named_bar_sync(10, 256);
+                if (words[2]) {
+                    // the last piece of the unit: all partial results are in memory
+                    __threadfence();
+                    const uint32_t r0 = min(half_tok, it.n_tok) * G, total = it.n_tok * G;
+                    for (uint32_t x = tid; x < total * (D / 4); x += 256) {
+                        const uint32_t row = x / (D / 4), c4 = x % (D / 4);
+                        const size_t at = (size_t)it.first_slot * 2 * kTile + (row < r0 ? row : kTile + row - r0);
+                        const float2 *ml = reinterpret_cast<const float2 *>(p.ml) + at;
+                        const float4 *acc = reinterpret_cast<const float4 *>(p.acc) + at * (D / 4) + c4;
+                        float m = kNegInf;
+                        for (uint32_t k = 0; k < it.n_parts; ++k) m = fmaxf(m, __ldcg(ml + (size_t)k * 2 * kTile).x);
+                        float sum = 0.f;
+                        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                        for (uint32_t k = 0; k < it.n_parts; ++k) {
+                            const float2 z = __ldcg(ml + (size_t)k * 2 * kTile);
+                            const float4 a = __ldcg(acc + (size_t)k * 2 * kTile * (D / 4));
+                            const float f = fast_exp2(z.x - m);
+                            if (f == 0.f) continue;
+                            sum += z.y * f;
+                            o.x += a.x * f;
+                            o.y += a.y * f;
+                            o.z += a.z * f;
+                            o.w += a.w * f;
+                        }
+                        const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+                        const uint32_t tk = row / G;
+                        *reinterpret_cast<uint2 *>(p.out + (it.tok0 + (uint64_t)tk) * p.out_stride_t +
+                                                   (uint64_t)(it.kvh * G + row % G) * p.out_stride_h + c4 * 4) =
+                            make_uint2(pack_f16x2(o.x * inv, o.y * inv), pack_f16x2(o.z * inv, o.w * inv));
+                    }
+                }
+                named_bar_sync(9, 256);  // words[2] and the partial rows are free again
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kQWarp) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
 }
 
 mf_status check_lens(MfContext *ctx, const uint32_t *q_lens, const uint32_t *kv_lens, uint32_t batch, uint64_t *tokens,
@@ -128,7 +678,10 @@ void mf_chunk_plan_destroy(MfContext *ctx, MfChunkPlan *pl)
         if (pl->staged[i]) cudaEventDestroy(pl->staged[i]);
         if (pl->pinned[i]) cudaFreeHost(pl->pinned[i]);
     }
-    if (pl->d_meta) cudaFree(pl->d_meta);
+    if (pl->d_list) cudaFree(pl->d_list);
+    if (pl->d_acc) cudaFree(pl->d_acc);
+    if (pl->d_ml) cudaFree(pl->d_ml);
+    if (pl->d_tickets) cudaFree(pl->d_tickets);
     delete pl;
 }
 
@@ -147,13 +700,21 @@ mf_status mf_chunk_plan_update(MfContext *ctx, MfChunkPlan *pl, const uint32_t *
     if ((st = check_cuda(ctx, cudaStreamIsCapturing(ctx->stream, &cap), "cudaStreamIsCapturing")) != MF_OK) return st;
     if (cap != cudaStreamCaptureStatusNone)
         return fail(ctx, MF_ERR_INVALID_OPERATION, "chunk plan: no update while the stream is being captured");
+    try {
+        build_chunk_plan(q_lens, kv_lens, pl->batch, pl->n_kv_heads, pl->n_heads / pl->n_kv_heads, pl->page_size, pl->window, pl->n_sinks,
+                         pl->n_ctas, pl->h_items, pl->h_begin);
+    } catch (const std::bad_alloc &) {
+        return fail(ctx, MF_ERR_OUT_OF_MEMORY, "chunk plan: host memory");
+    }
+    if (pl->h_items.size() > pl->item_capacity)
+        return fail(ctx, MF_ERR_INVALID_OPERATION, "chunk plan: %zu items, room for %llu", pl->h_items.size(), (unsigned long long)pl->item_capacity);
     const uint32_t s = pl->next_stage;
     if ((st = check_cuda(ctx, cudaEventSynchronize(pl->staged[s]), "chunk plan: staging")) != MF_OK) return st;
     uint32_t *w = pl->pinned[s];
-    w[0] = 0;
-    for (uint32_t b = 0; b < pl->batch; ++b) w[b + 1] = w[b] + q_lens[b];
-    for (uint32_t b = 0; b < pl->batch; ++b) w[pl->batch + 1 + b] = kv_lens[b];
-    st = check_cuda(ctx, cudaMemcpyAsync(pl->d_meta, w, 4 * (2 * (size_t)pl->batch + 1), cudaMemcpyHostToDevice, ctx->stream),
+    const size_t item_bytes = pl->h_items.size() * sizeof(ChunkItem);
+    memcpy(w, pl->h_begin.data(), 4 * pl->h_begin.size());
+    if (item_bytes) memcpy(w + pl->begin_words, pl->h_items.data(), item_bytes);
+    st = check_cuda(ctx, cudaMemcpyAsync(pl->d_list, w, 4 * (size_t)pl->begin_words + item_bytes, cudaMemcpyHostToDevice, ctx->stream),
                     "chunk plan: upload");
     if (st != MF_OK) return st;
     if ((st = check_cuda(ctx, cudaEventRecord(pl->staged[s], ctx->stream), "chunk plan: upload")) != MF_OK) return st;
@@ -200,12 +761,20 @@ mf_status mf_chunk_plan_create(MfContext *ctx, const uint32_t *q_lens, const uin
     auto ok = [&](cudaError_t r) {
         if (e == cudaSuccess) e = r;
     };
-    const size_t words = 2 * (size_t)batch + 1;
+    pl->n_ctas = (uint32_t)ctx->sm_count;
+    pl->begin_words = (pl->n_ctas + 1 + 15) / 16 * 16;
+    pl->item_capacity = chunk_item_capacity(batch, pl->max_tokens, n_kv_heads, n_heads / n_kv_heads, pl->n_ctas);
+    const size_t bytes = 4 * (size_t)pl->begin_words + pl->item_capacity * sizeof(ChunkItem);
     for (int i = 0; i < 2; ++i) {
-        ok(cudaMallocHost(reinterpret_cast<void **>(&pl->pinned[i]), 4 * words));
+        ok(cudaMallocHost(reinterpret_cast<void **>(&pl->pinned[i]), bytes));
         ok(cudaEventCreateWithFlags(&pl->staged[i], cudaEventDisableTiming));
     }
-    ok(cudaMalloc(reinterpret_cast<void **>(&pl->d_meta), 4 * words));
+    const size_t rows = (size_t)chunk_slots(pl->n_ctas) * 2 * kTile;
+    ok(cudaMalloc(reinterpret_cast<void **>(&pl->d_list), bytes));
+    ok(cudaMalloc(reinterpret_cast<void **>(&pl->d_acc), rows * head_dim * 4));
+    ok(cudaMalloc(reinterpret_cast<void **>(&pl->d_ml), rows * 8));
+    ok(cudaMalloc(reinterpret_cast<void **>(&pl->d_tickets), 4 * (size_t)pl->n_ctas));
+    if (e == cudaSuccess) ok(cudaMemsetAsync(pl->d_tickets, 0, 4 * (size_t)pl->n_ctas, ctx->stream));
     st = e == cudaSuccess ? mf_chunk_plan_update(ctx, pl, q_lens, kv_lens) : check_cuda(ctx, e, "chunk plan allocation");
     if (st != MF_OK) {
         mf_chunk_plan_destroy(ctx, pl);
@@ -247,28 +816,41 @@ mf_status mf_paged_chunk_attention(MfContext *ctx, const MfChunkPlan *pl, const 
     p.k_pool = static_cast<const __half *>(c->k_pool);
     p.v_pool = static_cast<const __half *>(c->v_pool);
     p.page_table = c->page_table;
-    p.q_begin = pl->d_meta;
-    p.kv_lens = pl->d_meta + pl->batch + 1;
+    p.list = pl->d_list;
+    p.acc = pl->d_acc;
+    p.ml = pl->d_ml;
+    p.tickets = pl->d_tickets;
+    p.begin_words = pl->begin_words;
     p.status = ctx->d_status;
     p.q_stride_t = a->q_stride_t;
     p.q_stride_h = a->q_stride_h;
     p.out_stride_t = a->out_stride_t;
     p.out_stride_h = a->out_stride_h;
-    p.batch = pl->batch;
-    p.n_heads = pl->n_heads;
     p.n_kv_heads = pl->n_kv_heads;
     p.group = pl->n_heads / pl->n_kv_heads;
-    p.page_size = pl->page_size;
+    for (p.page_shift = 0; (1u << p.page_shift) < pl->page_size; ++p.page_shift) {}
     p.pt_stride = c->page_table_stride;
     p.n_pages = c->n_pages;
     p.window = pl->window;
     p.n_sinks = pl->n_sinks;
-    p.scale_log2 = a->scale * 1.4426950408889634f;
-    const uint64_t blocks = ((uint64_t)pl->max_tokens * pl->n_heads + 7) / 8;
-    if (blocks > 0x7FFFFFFFull) return fail(ctx, MF_ERR_INVALID_SHAPE, "paged chunk attention: %u tokens", pl->max_tokens);
-    if (pl->head_dim == 128) chunk_rows_kernel<128><<<(uint32_t)blocks, 256, 0, ctx->stream>>>(p);
-    else chunk_rows_kernel<64><<<(uint32_t)blocks, 256, 0, ctx->stream>>>(p);
-    return check_launch(ctx, "chunk_rows_kernel");
+    // scale 0 (every visible key counts alike): a factor that keeps -inf * factor = -inf in the masked columns
+    p.scale_log2 = std::max(a->scale * 1.4426950408889634f, 1e-30f);
+    CUtensorMap tm_k, tm_v;
+    const uint64_t rows = (uint64_t)c->n_pages * c->n_kv_heads * c->page_size;
+    mf_status st = get_tensor_map(ctx, c->k_pool, rows, c->head_dim, c->page_size, 64, &tm_k, 2);
+    if (st == MF_OK) st = get_tensor_map(ctx, c->v_pool, rows, c->head_dim, c->page_size, 64, &tm_v, 2);
+    if (st != MF_OK) return st;
+    auto *kern = c->head_dim == 128 ? chunk_tc_kernel<128> : chunk_tc_kernel<64>;
+    const uint32_t smem = smem_bytes(c->head_dim);
+    static std::atomic<bool> configured[64][2];
+    const int di = c->head_dim == 128;
+    if (ctx->device >= 64 || !configured[ctx->device][di].load(std::memory_order_acquire)) {
+        st = check_cuda(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "cudaFuncSetAttribute(chunk_tc)");
+        if (st != MF_OK) return st;
+        if (ctx->device < 64) configured[ctx->device][di].store(true, std::memory_order_release);
+    }
+    kern<<<pl->n_ctas, kThreads, smem, ctx->stream>>>(tm_k, tm_v, p);
+    return check_launch(ctx, "chunk_tc_kernel");
 }
 
 }  // extern "C"

@@ -76,7 +76,21 @@ mf_status get_tensor_map(MfContext *ctx, const void *base, uint64_t rows, uint32
         return fail(ctx, MF_ERR_INVALID_SHAPE, "tensor-map box [%u x %u] unsupported", box_rows, box_cols);
     CUtensorMap tm;
     CUresult r;
-    if (whole_rows) {
+    if (whole_rows == 2) {
+        // (64 cols, 8 rows, column halves, 8-row groups of a page, pages x kv heads): the box is one (page, kv head) run
+        // and lands as [8-row group][half][8 rows][128 B], so that consecutive pages continue one evenly spaced
+        // sequence of 8-row groups whatever the page size.
+        if ((cols != 64 && cols != 128) || box_rows % 8 != 0 || rows % box_rows != 0)
+            return fail(ctx, MF_ERR_INVALID_SHAPE, "page tensor map [%u rows x %u cols] unsupported", box_rows, cols);
+        cuuint64_t gdim[5] = {64, 8, cols / 64, box_rows / 8, rows / box_rows};
+        cuuint64_t gstride[4] = {(cuuint64_t)cols * 2, 128, (cuuint64_t)cols * 16, (cuuint64_t)box_rows * cols * 2};
+        cuuint32_t box[5] = {64, 8, cols / 64, box_rows / 8, 1};
+        cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+        r = reinterpret_cast<EncodeTiledFn>(ctx->encode_fn)(
+            &tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void *>(base), gdim, gstride, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    } else if (whole_rows) {
         if (cols != 128) return fail(ctx, MF_ERR_INVALID_SHAPE, "whole-row tensor map needs 128 columns");
         // (64 cols, rows, 2 halves): the half index is the OUTER box dimension so that shared
         // memory receives [half][rows][128 B]; its global stride (128 B) is smaller than the row

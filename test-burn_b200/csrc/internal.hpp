@@ -271,6 +271,8 @@ inline __half *tensor_ptr(const MfTensor *t)
 // Cached f16 tensor map over [rows, cols] with the 128-byte swizzle.  whole_rows == 0: 2-D map,
 // box [box_rows, 64 cols].  whole_rows == 1 (cols == 128): 3-D map (64 cols, rows, 2 halves) whose
 // box [64, box_rows, 2] brings whole 256-byte rows in one copy, laid out [half][box_rows][128 B].
+// whole_rows == 2 (cols 64 or 128, box_rows = page size, rows = pages x kv heads x page size): 5-D map whose box is one
+// (page, kv head) run, laid out [8-row group][half][8 rows][128 B]; the last coordinate is page * kv heads + kv head.
 mf_status get_tensor_map(MfContext *ctx, const void *base, uint64_t rows, uint32_t cols,
                          uint32_t box_rows, uint32_t box_cols, CUtensorMap *out,
                          uint32_t whole_rows = 0);

@@ -115,6 +115,28 @@ __device__ __forceinline__ void tma_load_3d_hint(uint32_t dst, const void *tmap,
         : "memory");
 }
 
+// 5-D tiled tensor load of one box at (0, 0, 0, 0, w).
+__device__ __forceinline__ void tma_load_5d_last(uint32_t dst, const void *tmap, int32_t w, uint32_t bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %2, %2, %2, %3}], [%4];" ::"r"(dst),
+        "l"(tmap), "r"(0), "r"(w), "r"(bar)
+        : "memory");
+}
+
+// 16-byte asynchronous copy global -> shared, and the wait for all of this thread's.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async16_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+__device__ __forceinline__ void mbar_arrive_n(uint32_t bar, uint32_t count)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+
 __device__ __forceinline__ uint64_t l2_policy_evict_first()
 {
     uint64_t p;

@@ -1,0 +1,162 @@
+// Planner of a ragged batch's attention: which CTA walks which key tiles of which rows.
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "../../include/metallic_cuda.h"
+#include "../csrc/chunk_plan.hpp"
+
+namespace mf {
+namespace {
+
+// What an item costs its CTA beyond its tiles (loading q, draining the products, writing the rows), in tiles.
+constexpr uint32_t kItemCost = 2;
+// Shortest piece a unit is cut into when every CTA has several units.
+constexpr uint32_t kMinPiece = 2;
+
+}  // namespace
+
+uint64_t chunk_item_capacity(uint32_t batch, uint64_t max_tokens, uint32_t n_kv_heads, uint32_t group, uint32_t n_ctas)
+{
+    const uint32_t per_unit = 2 * (kChunkTile / group);
+    return (uint64_t)n_kv_heads * (std::min<uint64_t>(batch, max_tokens) + max_tokens / per_unit) + 2 * (uint64_t)n_ctas;
+}
+
+void build_chunk_plan(const uint32_t *q_lens, const uint32_t *kv_lens, uint32_t batch, uint32_t n_kv_heads, uint32_t group,
+                      uint32_t page_size, uint32_t window, uint32_t n_sinks, uint32_t n_ctas, std::vector<ChunkItem> &items,
+                      std::vector<uint32_t> &cta_begin)
+{
+    const uint32_t per_unit = 2 * (kChunkTile / group), P = page_size;
+    std::vector<ChunkItem> units;
+    uint64_t cost = 0;
+    uint32_t tok = 0;
+    for (uint32_t b = 0; b < batch; ++b) {
+        for (uint32_t h = 0; h < n_kv_heads; ++h)
+            for (uint32_t t = 0; t < q_lens[b]; t += per_unit) {
+                ChunkItem u{};
+                u.seq = b;
+                u.kvh = h;
+                u.tok0 = tok + t;
+                u.n_tok = std::min(per_unit, q_lens[b] - t);
+                u.pos0 = (int32_t)((int64_t)kv_lens[b] - q_lens[b] + t);
+                u.n_parts = 1;
+                const int64_t last = (int64_t)u.pos0 + u.n_tok - 1;
+                if (last >= 0) {
+                    const uint32_t first_pos = (uint32_t)std::max(u.pos0, 0);
+                    const uint32_t first_seen = window && first_pos >= window ? first_pos - window + 1 : 0;
+                    const uint32_t sinks = (uint32_t)std::min<int64_t>(n_sinks, last + 1);
+                    const uint32_t sink_pages = (sinks + P - 1) / P;
+                    u.first_page = first_seen / P;
+                    if (sink_pages >= u.first_page) u.first_page = 0;
+                    else u.n_sink_pages = sink_pages;
+                    u.n_pages = u.n_sink_pages + (uint32_t)(last / P) - u.first_page + 1;
+                    u.tile_end = (uint32_t)(((uint64_t)u.n_pages * P + kChunkTile - 1) / kChunkTile);
+                }
+                cost += u.tile_end + kItemCost;
+                units.push_back(u);
+            }
+        tok += q_lens[b];
+    }
+    items.clear();
+    cta_begin.assign(n_ctas + 1, 0);
+    uint32_t slots = 0, counters = 0;
+    // `parts` consecutive items of unit u are at the end of the list
+    auto number_parts = [&](size_t first) {
+        const uint32_t parts = (uint32_t)(items.size() - first);
+        if (parts < 2) return;
+        for (size_t i = first; i < items.size(); ++i) {
+            items[i].n_parts = parts;
+            items[i].first_slot = slots;
+            items[i].slot = slots + (uint32_t)(i - first);
+            items[i].counter = counters;
+        }
+        slots += parts;
+        ++counters;
+    };
+    // A span boundary usually cuts a unit, and the second piece pays for being an item again.
+    cost += (uint64_t)n_ctas * kItemCost;
+    uint32_t lo = 1;
+    bool pieces = units.size() <= n_ctas;
+    if (pieces) {
+        // Few units: one item per CTA, every unit cut into even pieces of at most `lo` tiles, the smallest number
+        // for which there are CTAs enough - unless unequal units leave some CTA more than an equal span would.
+        uint32_t hi = 1;
+        for (const ChunkItem &u : units) hi = std::max(hi, u.tile_end);
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            uint64_t need = 0;
+            for (const ChunkItem &u : units) need += std::max(1u, (u.tile_end + mid - 1) / mid);
+            if (need <= n_ctas) hi = mid;
+            else lo = mid + 1;
+        }
+        pieces = lo + kItemCost <= cost / n_ctas + 2;
+    }
+    if (pieces) {
+        for (const ChunkItem &u : units) {
+            const uint32_t parts = std::max(1u, (u.tile_end + lo - 1) / lo);
+            const size_t first = items.size();
+            for (uint32_t i = 0; i < parts; ++i) {
+                ChunkItem it = u;
+                it.tile_begin = (uint32_t)((uint64_t)u.tile_end * i / parts);
+                it.tile_end = (uint32_t)((uint64_t)u.tile_end * (i + 1) / parts);
+                items.push_back(it);
+            }
+            number_parts(first);
+        }
+        for (uint32_t c = 0; c <= n_ctas; ++c) cta_begin[c] = (uint32_t)std::min<size_t>(c, items.size());
+        return;
+    }
+    // Spans of equal cost over the list of units, cut where a span ends.
+    uint32_t cta = 0;
+    uint64_t before = 0;  // cost of everything placed so far
+    for (const ChunkItem &u : units) {
+        const size_t first = items.size();
+        uint32_t at = 0;
+        do {
+            // this CTA's span ends at cost * (cta + 1) / n_ctas
+            while (cta + 1 < n_ctas && before >= cost * (cta + 1) / n_ctas) cta_begin[++cta] = (uint32_t)items.size();
+            const uint64_t end = cost * (cta + 1) / n_ctas;
+            const uint64_t room = end > before + kItemCost ? end - before - kItemCost : 0;
+            uint32_t take = u.tile_end - at;
+            if (cta + 1 < n_ctas && take > room) {
+                take = (uint32_t)room;
+                if (take < kMinPiece || u.tile_end - at - take < kMinPiece) take = (uint64_t)take * 2 >= u.tile_end - at ? u.tile_end - at : 0;
+            }
+            if (take == 0 && u.tile_end > at) {  // too little room: the unit goes on in the next CTA
+                before = end;
+                continue;
+            }
+            ChunkItem it = u;
+            it.tile_begin = at;
+            it.tile_end = at + take;
+            items.push_back(it);
+            before += take + kItemCost;
+            at += take;
+        } while (at < u.tile_end);
+        number_parts(first);
+    }
+    while (cta < n_ctas) cta_begin[++cta] = (uint32_t)items.size();
+}
+
+}  // namespace mf
+
+extern "C" uint32_t mf_chunk_plan_build_host(const uint32_t *q_lens, const uint32_t *kv_lens, uint32_t batch, uint32_t n_heads,
+                                             uint32_t n_kv_heads, uint32_t page_size, uint32_t window, uint32_t n_sinks,
+                                             uint32_t n_ctas, uint32_t *items_out, uint32_t item_capacity, uint32_t *cta_begin_out)
+{
+    if (!q_lens || !kv_lens || !cta_begin_out || n_kv_heads == 0 || n_heads % n_kv_heads || n_heads / n_kv_heads == 0 ||
+        n_heads / n_kv_heads > 64 || page_size == 0 || n_ctas == 0)
+        return 0;
+    try {
+        std::vector<mf::ChunkItem> items;
+        std::vector<uint32_t> begin;
+        mf::build_chunk_plan(q_lens, kv_lens, batch, n_kv_heads, n_heads / n_kv_heads, page_size, window, n_sinks, n_ctas, items, begin);
+        if (items_out && items.size() <= item_capacity)
+            std::copy(reinterpret_cast<const uint32_t *>(items.data()),
+                      reinterpret_cast<const uint32_t *>(items.data() + items.size()), items_out);
+        std::copy(begin.begin(), begin.end(), cta_begin_out);
+        return (uint32_t)items.size();
+    } catch (const std::bad_alloc &) {
+        return 0;
+    }
+}
