@@ -15,7 +15,7 @@
 // works, the tensor pipe works for the other stream.  Nothing is handed from one group to the other between tiles.
 //
 //   warps 0-3, 4-7  softmax groups (one thread per row = TMEM lane)   warp 8   TMA producer, one copy per page and tile
-//   warps 9, 10     issue the products of streams 0, 1                warp 11  loads q, allocates TMEM
+//   warp 9          issues the products                               warp 10  loads q, allocates TMEM
 //
 // K and V tiles share one ring in the order in which the products want them.  A (page, kv head) run lands as
 // [8-row group][half][8 rows][128 bytes], so the 128 rows of a tile are evenly spaced 8-row groups whatever the page
@@ -45,18 +45,18 @@
 struct MfChunkPlan {
     uint32_t batch = 0, n_heads = 0, n_kv_heads = 0, head_dim = 0, page_size = 0, window = 0, n_sinks = 0;
     uint32_t max_tokens = 0, tokens = 0, max_pages = 0;
-    uint32_t n_ctas = 0, begin_words = 0;  // cta_begin, padded to whole items
+    uint32_t n_ctas = 0, begin_words = 0;  // cta_begin, padded to whole items; the last word is the number of tokens
     uint64_t item_capacity = 0;
     int device = 0;
     std::vector<mf::ChunkItem> h_items;
     std::vector<uint32_t> h_begin;
-    // [begin_words] cta_begin, [item_capacity] items; two pinned copies used in turn, each guarded by the event
+    // [begin_words], [item_capacity] items; two pinned copies used in turn, each guarded by the event
     // recorded after its upload
     uint32_t *d_list = nullptr;
     uint32_t *pinned[2] = {nullptr, nullptr};
     cudaEvent_t staged[2] = {nullptr, nullptr};
     uint32_t next_stage = 0;
-    float *d_acc = nullptr, *d_ml = nullptr;  // partial results: [slot][256 rows][D], [slot][256 rows][2]
+    float *d_acc = nullptr, *d_ml = nullptr;  // partial results: [slot][D / 4][256 rows][4], [slot][256 rows][2]
     uint32_t *d_tickets = nullptr;
 };
 
@@ -66,8 +66,8 @@ namespace {
 constexpr uint32_t kMaxGroup = 64;
 constexpr uint32_t kMaxLen = 1u << 30;  // positions and tile arithmetic stay inside 32 bits
 constexpr uint32_t kTile = kChunkTile;
-constexpr uint32_t kThreads = 384;
-constexpr uint32_t kProducerWarp = 8, kIssuerWarp = 9, kQWarp = 11;
+constexpr uint32_t kThreads = 352;
+constexpr uint32_t kProducerWarp = 8, kIssuerWarp = 9, kQWarp = 10;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr float kNegInf = -1e30f;
 constexpr float kRescaleThreshold = 8.0f;  // log2 of the largest weight kept in P
@@ -81,8 +81,8 @@ enum Bar : uint32_t {
     kOFull = 4,   // [2] the item's last P V has completed
     kOFree = 6,   // [2] the item's O has been read (8 arrivals)
     kQFull = 8,
-    kQFree = 9,   // 2 arrivals: the streams' last Q K^T of the item
-    kFull = 10    // [slots], then empty [slots] (2 arrivals: the streams)
+    kQFree = 9,   // the item's last Q K^T has completed
+    kFull = 10    // [slots], then empty [slots]
 };
 __host__ __device__ constexpr uint32_t num_bars(uint32_t d) { return kFull + 2 * ring_slots(d); }
 constexpr uint32_t kMlBytes = 2 * kTile * 8;  // (m, l) of the two streams' rows
@@ -102,6 +102,7 @@ struct ChunkParams {
     uint32_t *tickets, *status;
     uint64_t q_stride_t, q_stride_h, out_stride_t, out_stride_h;
     uint32_t begin_words, n_kv_heads, group, page_shift, pt_stride, n_pages, window, n_sinks;
+    uint32_t q_tokens;  // tokens that the maps of q cover; 0: q is loaded without them
     float scale_log2;
 };
 
@@ -147,9 +148,10 @@ __device__ __forceinline__ float max3(float a, float b, float c)
 // sum_x 2^(s_x - m) V[x][d0 .. d0 + dims) over the columns of the item that the row sees, key by key; one warp, result
 // in lanes * dims / 32 consecutive dims.  Rare: only for rows whose product with the whole tile was not finite.
 template <uint32_t D>
-__device__ __noinline__ void walk_row(const ChunkParams &p, const ChunkItem &it, const __half *q, int32_t pos, float m, uint32_t d0,
+__device__ __noinline__ void walk_row(const ChunkParams &p, uint32_t item, const __half *q, int32_t pos, float m, uint32_t d0,
                                       uint32_t dims, float (&acc)[D / 32])
 {
+    const ChunkItem it = load_item(p, item);
     const uint32_t lane = threadIdx.x & 31, E = dims / 32, P = 1u << p.page_shift;
     const Visible vis = visible(p, it, pos);
 #pragma unroll
@@ -186,7 +188,8 @@ __device__ __noinline__ void clear_rows(uint8_t *v_tile, int32_t dead0, int32_t 
 
 template <uint32_t D>
 __global__ void __launch_bounds__(kThreads, 1)
-chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ ChunkParams p)
+chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_q,
+                const __grid_constant__ CUtensorMap tm_q1, const __grid_constant__ ChunkParams p)
 {
     constexpr uint32_t kBytes = tile_bytes(D), kSlots = ring_slots(D);
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -212,10 +215,10 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             mbar_init(bar(kOFree + s), 8);
         }
         mbar_init(bar(kQFull), 1);
-        mbar_init(bar(kQFree), 2);
+        mbar_init(bar(kQFree), 1);
         for (uint32_t s = 0; s < kSlots; ++s) {
             mbar_init(bar(kFull + s), 1);
-            mbar_init(bar(kFull + kSlots + s), 2);
+            mbar_init(bar(kFull + kSlots + s), 1);
         }
         *abort_flag = 0;
         mbar_fence_init();
@@ -298,11 +301,29 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     } else if (warp == kQWarp) {
         // ------------------------------------------------------------------------- q (whole warp) ---
         uint32_t used = 0;
+        // A replayed launch can meet a plan with more tokens than q had when it was captured: then without the maps.
+        const bool by_map = __ldg(p.list + p.begin_words - 1) <= p.q_tokens;
         for (uint32_t i = item0; i < item1; ++i) {
             const ChunkItem it = load_item(p, i);
             if (it.tile_begin == it.tile_end) continue;
             if (used) wait(bar(kQFree), (used - 1) & 1, 4u);
             ++used;
+            if (by_map) {
+                // the tokens of a stream in one copy per column half; what lies behind the unit's is loaded too and
+                // computed on, and no one reads it
+                if (lane == 0) {
+                    const uint32_t streams = it.n_tok > half_tok ? 2 : 1, box = (it.n_tok == 1 ? 1 : half_tok) * G * 128;
+                    const CUtensorMap *tm = it.n_tok == 1 ? &tm_q1 : &tm_q;
+                    mbar_arrive_expect_tx(bar(kQFull), streams * (D / 64) * box);
+                    for (uint32_t x = 0; x < streams; ++x)
+#pragma unroll
+                        for (uint32_t h = 0; h < D / 64; ++h)
+                            tma_load_4d_box(q_smem + x * kBytes + h * kHalfTile, tm, 0, (int32_t)(it.kvh * G), (int32_t)(it.tok0 + x * half_tok),
+                                            (int32_t)h, bar(kQFull));
+                }
+                __syncwarp();
+                continue;
+            }
             constexpr uint32_t C = D / 8;
             const uint32_t rows = it.n_tok * G, per_stream = half_tok * G;
             for (uint32_t x = lane; x < rows * C; x += 32) {
@@ -318,72 +339,75 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(kQFull));
         }
-    } else if (warp >= kIssuerWarp) {
-        // ------------------------------------------------------------------ products of one stream ---
-        if (lane == 0) {
-            const uint32_t s = warp - kIssuerWarp;
+    } else if (warp == kIssuerWarp) {
+        // ------------------------------------------------------- the products of both streams (one warp) ---
+        // The streams take turns, P V of a tile and Q K^T of the stream's next one at a time: the softmax of one then
+        // runs while the tensor pipe works for the other.  (Issued by a thread each, the two blocks share the pipe, end
+        // together and leave it idle together: 6 000 cycles per pair of tiles instead of the sum of either half.)
+        {
+            const uint32_t elected = elect_one_sync();
             constexpr uint32_t kIdescQK = instr_desc_f16(kTile, kTile, 0), kIdescPV = instr_desc_f16(kTile, D, 1);
             constexpr uint32_t kGroupStride = 16 * D;  // bytes between 8-row groups of a K or V tile
-            const uint32_t s_tm = tmem + s * 128, o_tm = tmem + 256 + s * 128;
-            uint32_t slot = 0, phase = 0, q_phase = 0, p_phase = 0, o_uses = 0;
-            auto next_slot = [&]() {
-                if (++slot == kSlots) slot = 0, phase ^= 1;
+            uint32_t q_phase = 0, p_phase[2] = {0, 0}, o_uses[2] = {0, 0}, loads = 0;
+            auto full = [&](uint32_t load) {
+                wait(bar(kFull + load % kSlots), (load / kSlots) & 1, 16u);
+                return ring + load % kSlots * kBytes;
             };
-            auto skip = [&]() {  // a tile of the other stream
-                wait(bar(kFull + slot), phase, 8u);
-                mbar_arrive(bar(kFull + kSlots + slot));
-                next_slot();
-            };
+            auto release = [&](uint32_t load) { tc_commit_elected(elected, bar(kFull + kSlots + load % kSlots)); };
             for (uint32_t i = item0; i < item1; ++i) {
                 const ChunkItem it = load_item(p, i);
                 const uint32_t n = it.tile_end - it.tile_begin;
                 if (n == 0) continue;
                 const bool paired_rows = it.n_tok > half_tok;
-                const uint32_t step = paired_rows ? 1 : 2, mine = paired_rows ? n : (n + 1 - s) / 2;
-                const uint64_t q_desc = smem_desc(q_smem + (paired_rows ? s * kBytes : 0), 16, 1024);
-                wait(bar(kQFull), q_phase, 16u);
-                q_phase ^= 1;
-                if (mine == 0) mbar_arrive(bar(kQFree));
-                for (uint32_t j = 0, t = 0; t < n; ++j, t += step) {
-                    const bool two = step == 2 && t + 1 < n, own = paired_rows || s == 0 || two;
-                    if (step == 2 && s == 1) skip();
-                    if (own) {
-                        wait(bar(kFull + slot), phase, 16u);
-                        tc_fence_after();
-                        const uint64_t k_desc = smem_desc(ring + slot * kBytes, 16, kGroupStride);
+                const uint32_t tiles[2] = {paired_rows ? n : (n + 1) / 2, paired_rows ? n : n / 2};
+                auto scores = [&](uint32_t s, uint32_t j) {
+                    const uint32_t load = loads + (paired_rows ? 2 * j : 4 * j + s);
+                    const uint64_t k_desc = smem_desc(full(load), 16, kGroupStride);
+                    const uint64_t q_desc = smem_desc(q_smem + (paired_rows ? s * kBytes : 0), 16, 1024);
+                    tc_fence_after();
 #pragma unroll
-                        for (uint32_t kk = 0; kk < D / 16; ++kk)
-                            tc_mma_ss(s_tm, q_desc + (((kk >> 2) * kHalfTile + (kk & 3) * 32) >> 4),
-                                      k_desc + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4), kIdescQK, kk > 0);
-                        tc_commit(bar(kSFull + s));
-                        tc_commit(bar(kFull + kSlots + slot));
-                        if (j + 1 == mine) tc_commit(bar(kQFree));
-                        next_slot();
-                    }
-                    if (two && s == 0) skip();
-                    if (step == 2 && s == 1) skip();
-                    if (own) {
-                        wait(bar(kFull + slot), phase, 32u);
-                        wait(bar(kPFull + s), p_phase, 64u);
-                        p_phase ^= 1;
-                        if (j == 0 && o_uses) wait(bar(kOFree + s), (o_uses - 1) & 1, 128u);
+                    for (uint32_t kk = 0; kk < D / 16; ++kk)
+                        tc_mma_ss_elected(elected, tmem + s * 128, q_desc + (((kk >> 2) * kHalfTile + (kk & 3) * 32) >> 4),
+                                  k_desc + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4), kIdescQK, kk > 0);
+                    tc_commit_elected(elected, bar(kSFull + s));
+                    if (!paired_rows || s == 1) release(load);
+                };
+                wait(bar(kQFull), q_phase, 32u);
+                q_phase ^= 1;
+                scores(0, 0);
+                if (tiles[1]) scores(1, 0);
+                if (tiles[0] == 1) tc_commit_elected(elected, bar(kQFree));
+                for (uint32_t j = 0; j < tiles[0]; ++j)
+#pragma unroll
+                    for (uint32_t s = 0; s < 2; ++s) {
+                        if (j >= tiles[s]) continue;
+                        const uint32_t load = loads + (paired_rows ? 2 * j + 1 : 4 * j + (2 * j + 1 < n ? 2 + s : 1));
+                        const uint64_t v_desc = smem_desc(full(load), 1024, kGroupStride);
+                        wait(bar(kPFull + s), p_phase[s], 64u);
+                        p_phase[s] ^= 1;
+                        if (j == 0 && o_uses[s]) wait(bar(kOFree + s), (o_uses[s] - 1) & 1, 128u);
                         tc_fence_after();
-                        const uint64_t v_desc = smem_desc(ring + slot * kBytes, 1024, kGroupStride);
 #pragma unroll
                         for (uint32_t kk = 0; kk < kTile / 16; ++kk)
-                            tc_mma_ts(o_tm, s_tm + kk * 8, v_desc + ((kk * 2 * kGroupStride) >> 4), kIdescPV, (j > 0 || kk > 0) ? 1u : 0u);
-                        tc_commit(bar(kFull + kSlots + slot));
-                        if (j + 1 == mine) tc_commit(bar(kOFull + s));
-                        next_slot();
+                            tc_mma_ts_elected(elected, tmem + 256 + s * 128, tmem + s * 128 + kk * 8, v_desc + ((kk * 2 * kGroupStride) >> 4), kIdescPV,
+                                      (j > 0 || kk > 0) ? 1u : 0u);
+                        if (!paired_rows || s == 1) release(load);
+                        if (j + 1 == tiles[s]) {
+                            tc_commit_elected(elected, bar(kOFull + s));
+                        } else {
+                            scores(s, j + 1);
+                            // the last Q K^T of the item: stream 1's where it has as many tiles
+                            if (j + 2 == tiles[0] && s == (tiles[1] == tiles[0] ? 1u : 0u)) tc_commit_elected(elected, bar(kQFree));
+                        }
                     }
-                    if (two && s == 0) skip();
-                }
-                if (mine) ++o_uses;
+                ++o_uses[0];
+                o_uses[1] += tiles[1] > 0;
+                loads += 2 * n;
             }
             // The products have to be over before the TMEM goes back (they are, unless a wait ran out).
-            if (o_uses) wait(bar(kOFull + s), (o_uses - 1) & 1, 256u);
+            for (uint32_t s = 0; s < 2; ++s)
+                if (o_uses[s]) wait(bar(kOFull + s), (o_uses[s] - 1) & 1, 256u);
         }
-        __syncwarp();
     } else {
         // -------------------------------------------------------------- softmax groups / epilogue ---
         const uint32_t s = warp >> 2, quad = warp & 3, r_in = quad * 32 + lane, gtid = tid & 127;
@@ -391,8 +415,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         const uint32_t s_tm = tmem + lane_base + s * 128, o_base = tmem + lane_base + 256;
         uint32_t s_phase = 0, o_uses[2] = {0, 0}, loads = 0;  // loads: tiles the ring has seen before this item
         for (uint32_t i = item0; i < item1; ++i) {
-            const ChunkItem it = load_item(p, i);
-            const uint32_t n = it.tile_end - it.tile_begin;
+            ChunkItem it = load_item(p, i);
+            const uint32_t n = it.tile_end - it.tile_begin, x_item = it.tile_begin * kTile;
             const bool paired_rows = it.n_tok > half_tok;
             const uint32_t tok_first = paired_rows ? s * half_tok : 0;
             const uint32_t rows = min(half_tok, it.n_tok - tok_first) * G;
@@ -401,12 +425,13 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             const int32_t pos = it.pos0 + (int32_t)tok;
             const Visible vis = visible(p, it, pos);
             // columns that some row of the unit sees: [0, any_a), [any_b, any_c)
-            const Visible v_first = visible(p, it, max(it.pos0, 0)), v_last = visible(p, it, it.pos0 + (int32_t)it.n_tok - 1);
+            const Visible v_last = visible(p, it, it.pos0 + (int32_t)it.n_tok - 1);
+            const int32_t any_a = v_last.a, any_b = visible(p, it, max(it.pos0, 0)).b, any_c = v_last.c;
             const uint32_t mine = paired_rows ? n : (n + 1 - s) / 2;
             float m_ref = kNegInf, l = 0.f;
             for (uint32_t j = 0; j < mine; ++j) {
                 const uint32_t t = paired_rows ? j : 2 * j + s;
-                const int32_t x0 = (int32_t)((it.tile_begin + t) * kTile);
+                const int32_t x0 = (int32_t)(x_item + t * kTile);
                 wait(bar(kSFull + s), s_phase, 512u);
                 s_phase ^= 1;
                 tc_fence_after();
@@ -421,7 +446,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 #pragma unroll
                             for (uint32_t c = 0; c < kTile / 32; ++c) {
                                 const int32_t xc = x0 + (int32_t)c * 32;
-                                const uint32_t see = low_bits(vis.a - xc) | (low_bits(vis.c - xc) & ~low_bits(vis.b - xc));
+                                const uint32_t see = valid ? low_bits(vis.a - xc) | (low_bits(vis.c - xc) & ~low_bits(vis.b - xc)) : 0xFFFFFFFFu;
+                                if (__all_sync(0xffffffffu, see == 0xFFFFFFFFu)) continue;
 #pragma unroll
                                 for (uint32_t q = 0; q < 32; ++q)
                                     if (!((see >> q) & 1u)) r[c * 32 + q] = 0xFF800000u;  // -inf: weight exactly 0
@@ -478,8 +504,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                     l += acc.x + acc.y;
                 }
                 // Dead rows of this tile, relative to it: [any_a, any_b) and [any_c, end).
-                const int32_t end = (int32_t)kTile, gap0 = max(v_last.a - x0, 0), gap1 = min(v_first.b - x0, end);
-                const int32_t tail = v_last.c - x0;
+                const int32_t end = (int32_t)kTile, gap0 = max(any_a - x0, 0), gap1 = min(any_b - x0, end);
+                const int32_t tail = any_c - x0;
                 if (gap0 < gap1 || tail < end) {
                     uint32_t load = loads + (paired_rows ? 2 * j + 1 : 4 * j + ((2 * j + 1 < n) ? 2 + s : 1));
                     const uint32_t slot = load % kSlots;
@@ -494,6 +520,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                 if (lane == 0) mbar_arrive(bar(kPFull + s));
             }
             loads += 2 * n;
+            it = load_item(p, i);  // rather than kept in registers across the tiles
 
             // ---- the item's rows ------------------------------------------------------------------------
             // paired rows: group s has all D dims of its own rows; paired keys: dims [s * D/2, (s + 1) * D/2) of the
@@ -520,10 +547,21 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             f1 *= norm;
             const uint32_t d0 = paired_rows ? 0 : s * (D / 2), dims = paired_rows ? D : D / 2;
             const uint32_t slot_row = (paired_rows ? s * kTile : 0) + r_in;
-            float *part = p.acc + ((size_t)it.slot * 2 * kTile + slot_row) * D + d0;
+            // partial results lie by row inside a group of four dims, so that neighbouring threads write neighbouring words
+            float4 *part = reinterpret_cast<float4 *>(p.acc) + ((size_t)it.slot * (D / 4) + d0 / 4) * (2 * kTile) + slot_row;
             __half *dst = p.out + (it.tok0 + (uint64_t)tok) * p.out_stride_t + (uint64_t)head * p.out_stride_h + d0;
-            bool odd = false;  // a value that is not finite although the sum of the weights is
+            float odd = 0.f;  // NaN: a value that is not finite
             if (busy) {
+                // Rows go out four lanes to a row: the lanes of a quad swap their 16-byte blocks, lane q then has block q
+                // of each of the quad's rows and four lanes store 64 consecutive bytes.
+                __half *quad_dst[4];
+                bool quad_valid[4];
+#pragma unroll
+                for (uint32_t t = 0; t < 4; ++t) {
+                    const uint32_t src = (lane & ~3u) + t;
+                    quad_dst[t] = reinterpret_cast<__half *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), src)) + (lane & 3) * 8;
+                    quad_valid[t] = __shfl_sync(0xffffffffu, (uint32_t)valid, src) != 0;
+                }
 #pragma unroll 1
                 for (uint32_t c = 0; c < dims / 32; ++c) {
                     float o[32];
@@ -533,30 +571,46 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                         tmem_ld32(o_base + (paired_rows ? s * 128 : 0) + d0 + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
                         tc_wait_ld();
 #pragma unroll
-                        for (uint32_t q = 0; q < 32; ++q) o[q] = f0 == 0.f ? 0.f : o[q] * f0;
+                        for (uint32_t q = 0; q < 32; ++q) o[q] *= f0;
                         if (!paired_rows && n > 1) {
                             uint32_t o1[32];
                             tmem_ld32(o_base + 128 + d0 + c * 32, o1);
                             tc_wait_ld();
 #pragma unroll
-                            for (uint32_t q = 0; q < 32; ++q) o[q] += f1 == 0.f ? 0.f : __uint_as_float(o1[q]) * f1;
+                            for (uint32_t q = 0; q < 32; ++q) o[q] = fmaf(__uint_as_float(o1[q]), f1, o[q]);
                         }
                     }
-                    if (valid) {
 #pragma unroll
-                        for (uint32_t q = 0; q < 32; ++q) odd |= !(fabsf(o[q]) <= 3.0e38f);
-                        if (cut) {
+                    for (uint32_t q = 0; q < 32; ++q) odd = fmaf(o[q], 0.f, odd);
+                    if (cut) {
+                        if (valid) {
 #pragma unroll
                             for (uint32_t q = 0; q < 32; q += 4)
-                                __stcg(reinterpret_cast<float4 *>(part + c * 32 + q), make_float4(o[q], o[q + 1], o[q + 2], o[q + 3]));
-                        } else {
+                                __stcg(part + (c * 8 + q / 4) * (2 * kTile), make_float4(o[q], o[q + 1], o[q + 2], o[q + 3]));
+                        }
+                        continue;
+                    }
+                    uint32_t w[16];
 #pragma unroll
-                            for (uint32_t q = 0; q < 32; q += 8)
-                                *reinterpret_cast<uint4 *>(dst + c * 32 + q) =
-                                    make_uint4(pack_f16x2(o[q], o[q + 1]), pack_f16x2(o[q + 2], o[q + 3]), pack_f16x2(o[q + 4], o[q + 5]),
-                                               pack_f16x2(o[q + 6], o[q + 7]));
+                    for (uint32_t q = 0; q < 16; ++q) w[q] = pack_f16x2(o[2 * q], o[2 * q + 1]);
+#pragma unroll
+                    for (uint32_t bit = 1; bit <= 2; bit <<= 1) {
+                        const bool upper = lane & bit;
+#pragma unroll
+                        for (uint32_t t = 0; t < 4; ++t) {
+                            if (t & bit) continue;
+#pragma unroll
+                            for (uint32_t e = 0; e < 4; ++e) {
+                                const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? w[t * 4 + e] : w[(t | bit) * 4 + e], bit);
+                                if (upper) w[t * 4 + e] = got;
+                                else w[(t | bit) * 4 + e] = got;
+                            }
                         }
                     }
+#pragma unroll
+                    for (uint32_t t = 0; t < 4; ++t)
+                        if (quad_valid[t])
+                            *reinterpret_cast<uint4 *>(quad_dst[t] + c * 32) = make_uint4(w[t * 4], w[t * 4 + 1], w[t * 4 + 2], w[t * 4 + 3]);
                 }
             }
             // O has been read: the next item's first product may overwrite it.
@@ -572,20 +626,20 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             }
             if (act0 || (paired_rows && n)) ++o_uses[0];
             if (act1 || (paired_rows && n)) ++o_uses[1];
-            uint32_t again = __ballot_sync(0xffffffffu, odd && fabsf(l) <= 3.0e38f && fabsf(m_ref) <= 3.0e38f);
+            uint32_t again = __ballot_sync(0xffffffffu, valid && !(odd == 0.f) && fabsf(l) <= 3.0e38f && fabsf(m_ref) <= 3.0e38f);
             while (again) {
                 const uint32_t src = __ffs(again) - 1;
                 again &= again - 1;
                 const uint32_t w_tok = __shfl_sync(0xffffffffu, tok, src), w_head = __shfl_sync(0xffffffffu, head, src);
                 const float w_m = __shfl_sync(0xffffffffu, m_ref, src), w_norm = __shfl_sync(0xffffffffu, norm, src);
                 float acc[D / 32];
-                walk_row<D>(p, it, p.q + (it.tok0 + (uint64_t)w_tok) * p.q_stride_t + (uint64_t)w_head * p.q_stride_h, it.pos0 + (int32_t)w_tok,
+                walk_row<D>(p, i, p.q + (it.tok0 + (uint64_t)w_tok) * p.q_stride_t + (uint64_t)w_head * p.q_stride_h, it.pos0 + (int32_t)w_tok,
                             w_m, d0, dims, acc);
                 const uint32_t E = dims / 32;
                 for (uint32_t e = 0; e < E; ++e) {
                     const uint32_t d = lane * E + e;
                     if (cut)
-                        __stcg(p.acc + ((size_t)it.slot * 2 * kTile + (paired_rows ? s * kTile : 0) + quad * 32 + src) * D + d0 + d, acc[e]);
+                        __stcg(p.acc + (((size_t)it.slot * (D / 4) + (d0 + d) / 4) * (2 * kTile) + (paired_rows ? s * kTile : 0) + quad * 32 + src) * 4 + d % 4, acc[e]);
                     else
                         p.out[(it.tok0 + (uint64_t)w_tok) * p.out_stride_t + (uint64_t)w_head * p.out_stride_h + d0 + d] = __float2half_rn(acc[e] * w_norm);
                 }
@@ -605,33 +659,40 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                 if (words[2]) {
                     // the last piece of the unit: all partial results are in memory
                     __threadfence();
+                    // a thread takes 16 dims of a row; everything a piece has for it is requested at once
                     const uint32_t r0 = min(half_tok, it.n_tok) * G, total = it.n_tok * G;
-                    for (uint32_t x = tid; x < total * (D / 4); x += 256) {
-                        const uint32_t row = x / (D / 4), c4 = x % (D / 4);
-                        const size_t at = (size_t)it.first_slot * 2 * kTile + (row < r0 ? row : kTile + row - r0);
-                        const float2 *ml = reinterpret_cast<const float2 *>(p.ml) + at;
-                        const float4 *acc = reinterpret_cast<const float4 *>(p.acc) + at * (D / 4) + c4;
-                        float m = kNegInf;
-                        for (uint32_t k = 0; k < it.n_parts; ++k) m = fmaxf(m, __ldcg(ml + (size_t)k * 2 * kTile).x);
-                        float sum = 0.f;
-                        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+                    for (uint32_t x = tid; x < total * (D / 16); x += 256) {
+                        const uint32_t grp = x / total, row = x - grp * total, sr = row < r0 ? row : kTile + row - r0;
+                        const float2 *ml = reinterpret_cast<const float2 *>(p.ml) + (size_t)it.first_slot * (2 * kTile) + sr;
+                        const float4 *acc = reinterpret_cast<const float4 *>(p.acc) + ((size_t)it.first_slot * (D / 4) + grp * 4) * (2 * kTile) + sr;
+                        float m = kNegInf, sum = 0.f, o[16];
+#pragma unroll
+                        for (uint32_t e = 0; e < 16; ++e) o[e] = 0.f;
+#pragma unroll 2
                         for (uint32_t k = 0; k < it.n_parts; ++k) {
-                            const float2 z = __ldcg(ml + (size_t)k * 2 * kTile);
-                            const float4 a = __ldcg(acc + (size_t)k * 2 * kTile * (D / 4));
-                            const float f = fast_exp2(z.x - m);
-                            if (f == 0.f) continue;
-                            sum += z.y * f;
-                            o.x += a.x * f;
-                            o.y += a.y * f;
-                            o.z += a.z * f;
-                            o.w += a.w * f;
+                            const float2 z = __ldcg(ml + (size_t)k * (2 * kTile));
+                            float4 a[4];
+#pragma unroll
+                            for (uint32_t e = 0; e < 4; ++e) a[e] = __ldcg(acc + ((size_t)k * (D / 4) + e) * (2 * kTile));
+                            const float m_new = fmaxf(m, z.x), f_old = fast_exp2(m - m_new), f = fast_exp2(z.x - m_new);
+                            m = m_new;
+                            sum = fmaf(z.y, f, sum * f_old);
+#pragma unroll
+                            for (uint32_t e = 0; e < 4; ++e) {
+                                o[4 * e] = fmaf(a[e].x, f, o[4 * e] * f_old);
+                                o[4 * e + 1] = fmaf(a[e].y, f, o[4 * e + 1] * f_old);
+                                o[4 * e + 2] = fmaf(a[e].z, f, o[4 * e + 2] * f_old);
+                                o[4 * e + 3] = fmaf(a[e].w, f, o[4 * e + 3] * f_old);
+                            }
                         }
                         const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
                         const uint32_t tk = row / G;
-                        *reinterpret_cast<uint2 *>(p.out + (it.tok0 + (uint64_t)tk) * p.out_stride_t +
-                                                   (uint64_t)(it.kvh * G + row % G) * p.out_stride_h + c4 * 4) =
-                            make_uint2(pack_f16x2(o.x * inv, o.y * inv), pack_f16x2(o.z * inv, o.w * inv));
+                        uint4 *to = reinterpret_cast<uint4 *>(p.out + (it.tok0 + (uint64_t)tk) * p.out_stride_t +
+                                                              (uint64_t)(it.kvh * G + row - tk * G) * p.out_stride_h + grp * 16);
+#pragma unroll
+                        for (uint32_t e = 0; e < 2; ++e)
+                            to[e] = make_uint4(pack_f16x2(o[8 * e] * inv, o[8 * e + 1] * inv), pack_f16x2(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                                               pack_f16x2(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack_f16x2(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
                     }
                 }
                 named_bar_sync(9, 256);  // words[2] and the partial rows are free again
@@ -713,6 +774,7 @@ mf_status mf_chunk_plan_update(MfContext *ctx, MfChunkPlan *pl, const uint32_t *
     uint32_t *w = pl->pinned[s];
     const size_t item_bytes = pl->h_items.size() * sizeof(ChunkItem);
     memcpy(w, pl->h_begin.data(), 4 * pl->h_begin.size());
+    w[pl->begin_words - 1] = (uint32_t)tokens;
     if (item_bytes) memcpy(w + pl->begin_words, pl->h_items.data(), item_bytes);
     st = check_cuda(ctx, cudaMemcpyAsync(pl->d_list, w, 4 * (size_t)pl->begin_words + item_bytes, cudaMemcpyHostToDevice, ctx->stream),
                     "chunk plan: upload");
@@ -762,7 +824,7 @@ mf_status mf_chunk_plan_create(MfContext *ctx, const uint32_t *q_lens, const uin
         if (e == cudaSuccess) e = r;
     };
     pl->n_ctas = (uint32_t)ctx->sm_count;
-    pl->begin_words = (pl->n_ctas + 1 + 15) / 16 * 16;
+    pl->begin_words = (pl->n_ctas + 2 + 15) / 16 * 16;
     pl->item_capacity = chunk_item_capacity(batch, pl->max_tokens, n_kv_heads, n_heads / n_kv_heads, pl->n_ctas);
     const size_t bytes = 4 * (size_t)pl->begin_words + pl->item_capacity * sizeof(ChunkItem);
     for (int i = 0; i < 2; ++i) {
@@ -840,6 +902,19 @@ mf_status mf_paged_chunk_attention(MfContext *ctx, const MfChunkPlan *pl, const 
     mf_status st = get_tensor_map(ctx, c->k_pool, rows, c->head_dim, c->page_size, 64, &tm_k, 2);
     if (st == MF_OK) st = get_tensor_map(ctx, c->v_pool, rows, c->head_dim, c->page_size, 64, &tm_v, 2);
     if (st != MF_OK) return st;
+    // q as (64 columns, heads, tokens, column halves): a box is the kv head's query heads of a stream's tokens (tm_q) or of
+    // one token (tm_q1) and lands as rows (token, head) of 128 bytes
+    CUtensorMap tm_q{}, tm_q1{};
+    if (pl->tokens) {
+        const uint64_t dims[4] = {64, pl->n_heads, pl->tokens, c->head_dim / 64};
+        const uint64_t strides[3] = {a->q_stride_h * 2, a->q_stride_t * 2, 128};
+        const uint32_t box[4] = {64, p.group, kTile / p.group, 1}, box1[4] = {64, p.group, 1, 1};
+        bool ok = false, ok1 = false;
+        st = encode_f16_map(ctx, &tm_q, a->q, 4, dims, strides, box, &ok);
+        if (st == MF_OK) st = encode_f16_map(ctx, &tm_q1, a->q, 4, dims, strides, box1, &ok1);
+        if (st != MF_OK) return st;
+        if (ok && ok1) p.q_tokens = pl->tokens;
+    }
     auto *kern = c->head_dim == 128 ? chunk_tc_kernel<128> : chunk_tc_kernel<64>;
     const uint32_t smem = smem_bytes(c->head_dim);
     static std::atomic<bool> configured[64][2];
@@ -849,7 +924,7 @@ mf_status mf_paged_chunk_attention(MfContext *ctx, const MfChunkPlan *pl, const 
         if (st != MF_OK) return st;
         if (ctx->device < 64) configured[ctx->device][di].store(true, std::memory_order_release);
     }
-    kern<<<pl->n_ctas, kThreads, smem, ctx->stream>>>(tm_k, tm_v, p);
+    kern<<<pl->n_ctas, kThreads, smem, ctx->stream>>>(tm_k, tm_v, tm_q, tm_q1, p);
     return check_launch(ctx, "chunk_tc_kernel");
 }
 

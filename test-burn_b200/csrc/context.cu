@@ -53,6 +53,38 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t
                                   CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
                                   CUtensorMapFloatOOBfill);
 
+static mf_status find_encode_fn(MfContext *ctx)
+{
+    if (ctx->encode_fn) return MF_OK;
+    cudaDriverEntryPointQueryResult q;
+    void *fn = nullptr;
+    cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
+    if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || !fn)
+        return fail(ctx, MF_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available");
+    ctx->encode_fn = fn;
+    return MF_OK;
+}
+
+mf_status encode_f16_map(MfContext *ctx, CUtensorMap *out, const void *base, uint32_t rank, const uint64_t *dims,
+                         const uint64_t *strides, const uint32_t *box, bool *encoded)
+{
+    const mf_status st = find_encode_fn(ctx);
+    if (st != MF_OK) return st;
+    cuuint64_t gdim[5], gstride[4];
+    cuuint32_t b[5], estr[5];
+    for (uint32_t i = 0; i < rank; ++i) {
+        gdim[i] = dims[i];
+        b[i] = box[i];
+        estr[i] = 1;
+        if (i + 1 < rank) gstride[i] = strides[i];
+    }
+    *encoded = reinterpret_cast<EncodeTiledFn>(ctx->encode_fn)(
+                   out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void *>(base), gdim, gstride, b, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return MF_OK;
+}
+
 mf_status get_tensor_map(MfContext *ctx, const void *base, uint64_t rows, uint32_t cols, uint32_t box_rows,
                          uint32_t box_cols, CUtensorMap *out, uint32_t whole_rows)
 {
@@ -62,14 +94,8 @@ mf_status get_tensor_map(MfContext *ctx, const void *base, uint64_t rows, uint32
         *out = it->second;
         return MF_OK;
     }
-    if (!ctx->encode_fn) {
-        cudaDriverEntryPointQueryResult q;
-        void *fn = nullptr;
-        cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
-        if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || !fn)
-            return fail(ctx, MF_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available");
-        ctx->encode_fn = fn;
-    }
+    const mf_status found = find_encode_fn(ctx);
+    if (found != MF_OK) return found;
     if (reinterpret_cast<uintptr_t>(base) & 15u)
         return fail(ctx, MF_ERR_INVALID_SHAPE, "K/V base pointer must be 16-byte aligned");
     if (box_cols * 2 != 128 || cols % box_cols != 0 || box_rows == 0 || box_rows > 256)

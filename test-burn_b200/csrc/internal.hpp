@@ -277,6 +277,11 @@ mf_status get_tensor_map(MfContext *ctx, const void *base, uint64_t rows, uint32
                          uint32_t box_rows, uint32_t box_cols, CUtensorMap *out,
                          uint32_t whole_rows = 0);
 
+// f16 tensor map with the 128-byte swizzle, up to 5 dimensions (strides in bytes, of dimensions 1 and up).  *encoded:
+// whether the driver takes these strides.
+mf_status encode_f16_map(MfContext *ctx, CUtensorMap *out, const void *base, uint32_t rank, const uint64_t *dims,
+                         const uint64_t *strides, const uint32_t *box, bool *encoded);
+
 mf_status ensure_scratch(MfContext *ctx, uint64_t bytes);
 
 // Host planner: cut the tiles of all (sequence, kv head) units into n_ctas equal spans.

@@ -125,6 +125,16 @@ __device__ __forceinline__ void tma_load_5d_last(uint32_t dst, const void *tmap,
         : "memory");
 }
 
+// 4-D tiled tensor load of one box.
+__device__ __forceinline__ void tma_load_4d_box(uint32_t dst, const void *tmap, int32_t x, int32_t y, int32_t z, int32_t w, uint32_t bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        : "memory");
+}
+
 // 16-byte asynchronous copy global -> shared, and the wait for all of this thread's.
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src)
 {
