@@ -550,10 +550,9 @@ class Foundry:
         """Causal (windowed) attention of the plan's new tokens; q and out: f16 [tokens, Hq*D] or [tokens, Hq, D], any
         token and head strides that are multiples of 8."""
         d = cache.head_dim
-        _check_rows(q, plan, d, "q")
-        _check_rows(out, plan, d, "out")
-        a = MfPagedChunkArgs(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1) if q.dim() == 3 else d, out.stride(0),
-                             out.stride(1) if out.dim() == 3 else d, 1.0 / math.sqrt(d) if scale is None else scale)
+        qt, qh = _head_strides(q, plan, d, "q")
+        ot, oh = _head_strides(out, plan, d, "out")
+        a = MfPagedChunkArgs(q.data_ptr(), out.data_ptr(), qt, qh, ot, oh, d ** -0.5 if scale is None else scale)
         self.check(lib.mf_paged_chunk_attention(self._h, plan._h, C.byref(cache), C.byref(a)))
 
     def paged_mrope_append(self, cache, q, k, v, q_rot, cos, sin, positions, q_begin, axes, *, n_heads,
@@ -561,25 +560,25 @@ class Foundry:
         """Rotate q and k of a ragged batch by positions on several axes and append k, v to the pages of an f16 or an
         8-bit cache.  q, k, v, q_rot: f16 [tokens, heads*D] (rows may be strided; q and q_rot may be None), positions:
         int32 [n_axes, tokens], q_begin: int32 [batch + 1], axes: the axis of every frequency (see mrope_axes)."""
-        d, tokens = cache.head_dim, k.shape[0]
-        heads = (("q", q, n_heads), ("k", k, cache.n_kv_heads), ("v", v, cache.n_kv_heads), ("q_rot", q_rot, n_heads))
-        for name, x, h in heads:
-            if x is not None and (x.dim() != 2 or x.shape[0] != tokens or x.shape[1] != h * d or x.stride(1) != 1
-                                  or x.element_size() != 2):
-                raise MetalError(2, f"mrope append: {name} must be f16 [{tokens}, {h * d}] with unit column stride")
-        if cos.shape[1] * 2 != d or sin.shape != cos.shape or not (cos.is_contiguous() and sin.is_contiguous()):
-            raise MetalError(2, f"mrope append: cos / sin must be [rows, {d // 2}]")
-        if positions.dim() != 2 or positions.shape[1] != tokens or positions.stride(1) != 1 or positions.element_size() != 4:
+        d, tokens, n_kv = cache.head_dim, k.shape[0], cache.n_kv_heads
+        half = d // 2
+        k_stride, v_stride = _row_stride(k, tokens, n_kv * d, "k"), _row_stride(v, tokens, n_kv * d, "v")
+        q_stride = _row_stride(q, tokens, n_heads * d, "q") if q is not None else 0
+        rot_stride = _row_stride(q_rot, tokens, n_heads * d, "q_rot") if q_rot is not None else 0
+        rows = cos.shape[0]
+        if cos.shape != (rows, half) or sin.shape != (rows, half) or not (cos.is_contiguous() and sin.is_contiguous()):
+            raise MetalError(2, f"mrope append: cos / sin must be [rows, {half}]")
+        p_strides = positions.stride()
+        if len(p_strides) != 2 or positions.shape[1] != tokens or p_strides[1] != 1 or positions.element_size() != 4:
             raise MetalError(2, f"mrope append: positions must be int32 [n_axes, {tokens}]")
-        if q_begin.numel() != cache.batch + 1 or q_begin.element_size() != 4 or not q_begin.is_contiguous():
+        if q_begin.shape != (cache.batch + 1,) or q_begin.element_size() != 4 or q_begin.stride() != (1,):
             raise MetalError(2, f"mrope append: q_begin must be int32 [{cache.batch + 1}]")
-        if len(axes) != d // 2:
-            raise MetalError(2, f"mrope append: {len(axes)} axes for {d // 2} frequencies")
+        if len(axes) != half:
+            raise MetalError(2, f"mrope append: {len(axes)} axes for {half} frequencies")
         n_axes = positions.shape[0]
         a = MfMropeAppendArgs(_ptr(q), k.data_ptr(), v.data_ptr(), _ptr(q_rot), cos.data_ptr(), sin.data_ptr(),
-                              positions.data_ptr(), q_begin.data_ptr(), 0 if q is None else q.stride(0), k.stride(0), v.stride(0),
-                              0 if q_rot is None else q_rot.stride(0), tokens, n_heads, n_axes,
-                              positions.stride(0) if n_axes > 1 else tokens, cos.shape[0], rope_mode)
+                              positions.data_ptr(), q_begin.data_ptr(), q_stride, k_stride, v_stride, rot_stride, tokens, n_heads,
+                              n_axes, p_strides[0] if n_axes > 1 else tokens, rows, rope_mode)
         C.memmove(a.axis, bytes(axes), len(axes))
         fn = lib.mf_paged_kv8_mrope_append if isinstance(cache, MfPagedKv8) else lib.mf_paged_mrope_append
         self.check(fn(self._h, C.byref(cache), C.byref(a)))
@@ -905,10 +904,23 @@ class ChunkPlan:
             pass
 
 
-def _check_rows(x, plan: ChunkPlan, d: int, name: str):
-    cols = tuple(x.shape[1:])
-    if x.shape[0] < plan.tokens or cols not in ((plan.n_heads * d,), (plan.n_heads, d)) or x.stride(-1) != 1 or x.element_size() != 2:
-        raise MetalError(2, f"paged chunk attention: {name} {tuple(x.shape)} for {plan.tokens} tokens of {plan.n_heads} heads of {d}")
+def _head_strides(x, plan: ChunkPlan, d: int, name: str):
+    """(token, head) strides of f16 [tokens, heads * d] or [tokens, heads, d]."""
+    shape, st = x.shape, x.stride()
+    if shape[0] >= plan.tokens and st[-1] == 1 and x.element_size() == 2:
+        if len(shape) == 2 and shape[1] == plan.n_heads * d:
+            return st[0], d
+        if len(shape) == 3 and shape[1] == plan.n_heads and shape[2] == d:
+            return st[0], st[1]
+    raise MetalError(2, f"paged chunk attention: {name} {tuple(shape)} for {plan.tokens} tokens of {plan.n_heads} heads of {d}")
+
+
+def _row_stride(x, rows: int, cols: int, name: str) -> int:
+    """Row stride of f16 [rows, cols] with unit column stride."""
+    st = x.stride()
+    if x.shape != (rows, cols) or st[1] != 1 or x.element_size() != 2:
+        raise MetalError(2, f"mrope append: {name} must be f16 [{rows}, {cols}] with unit column stride")
+    return st[0]
 
 
 def mrope_axes(sections, interleaved: bool = False) -> bytes:

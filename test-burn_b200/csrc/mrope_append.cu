@@ -4,7 +4,11 @@
 // tokens, not positions.  Products and sums in f32 from f16 operands, one rounding to f16 (append.cuh); the 8-bit
 // cache quantises the rounded K row and the V row: scale = max|x| / 448, byte = e4m3(x / scale).
 //
-// One warp per (token, head slot).
+// Bound by HBM: every row is read once and written once.  A CTA has the new tokens of one sequence that fall into one
+// aligned block of cache rows (8 rows; 16 for the 8-bit cache, whose V bytes lie in 16-row blocks): it gathers the cos /
+// sin rows of its tokens into shared memory once for all heads, and finds its sequence once.  A thread turns two 16-byte
+// chunks at a time (append.cuh), several in flight.  V bytes of the 8-bit cache are transposed through shared memory: a
+// whole block goes out as 16-byte words, a part of one byte by byte.
 #include <cuda_fp8.h>
 
 #include "append.cuh"
@@ -26,101 +30,181 @@ struct MropeParams {
     uint8_t axis[64];
 };
 
-// Byte of (row r of the page, dim d) in the dim-major 16-key blocks of a V page of 128-wide heads.
-__device__ __forceinline__ uint32_t v_block_offset(uint32_t r, uint32_t d) { return (r / 16) * 2048 + d * 16 + r % 16; }
-
-template <bool K8>
-__global__ void __launch_bounds__(256) mrope_append_kernel(const __grid_constant__ MropeParams p)
+// scale of the 128-wide row whose chunk pairs eight neighbouring threads hold; every lane of the warp takes part
+__device__ __forceinline__ float row_scale(const Chunk &a, const Chunk &c, bool live)
 {
-    const uint32_t lane = threadIdx.x & 31, D = p.head_dim;
-    const uint64_t wid = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-    const uint32_t q_slots = p.q_rot ? p.n_heads : 0, slots = q_slots + 2 * p.n_kv_heads;
-    if (wid >= (uint64_t)p.tokens * slots) return;
-    const uint32_t t = (uint32_t)(wid / slots), slot = (uint32_t)(wid % slots);
-    const bool is_q = slot < q_slots, is_v = slot >= q_slots + p.n_kv_heads;
-    const uint32_t head = is_q ? slot : (is_v ? slot - q_slots - p.n_kv_heads : slot - q_slots);
-    const __half *src = is_q ? p.q + t * p.q_stride + head * D : is_v ? p.v + t * p.v_stride + head * D : p.k + t * p.k_stride + head * D;
-    __half x[2], y[2];
-    __half a[2][2];  // pairs lane and lane + 32: (first, second)
-    const uint32_t half = D / 2;
-    auto dim = [&](uint32_t pr, uint32_t second) { return p.rope_mode == MF_ROPE_MODE_NEOX ? pr + second * half : 2 * pr + second; };
-#pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
-        const uint32_t pr = lane + 32 * i;
-        a[i][0] = a[i][1] = __float2half_rn(0.f);
-        if (pr >= half) continue;
-        x[0] = src[dim(pr, 0)];
-        x[1] = src[dim(pr, 1)];
-        y[0] = x[0];
-        y[1] = x[1];
-        if (!is_v) {
-            const uint32_t row = p.positions[(size_t)p.axis[pr] * p.pos_stride + t];
-            if (row >= p.table_rows) {
-                atomicOr(p.status, kStatusBadPage);
-            } else {
-                const float c = __half2float(p.cos_t[(size_t)row * half + pr]), s = __half2float(p.sin_t[(size_t)row * half + pr]);
-                y[0] = rot_first(__half2float(x[0]), __half2float(x[1]), c, s);
-                y[1] = rot_second(__half2float(x[0]), __half2float(x[1]), c, s);
-            }
-        }
-        a[i][0] = y[0];
-        a[i][1] = y[1];
-    }
-    if (is_q) {
-        __half *dst = p.q_rot + t * p.q_rot_stride + head * D;
-#pragma unroll
-        for (uint32_t i = 0; i < 2; ++i)
-            if (lane + 32 * i < half) {
-                dst[dim(lane + 32 * i, 0)] = a[i][0];
-                dst[dim(lane + 32 * i, 1)] = a[i][1];
-            }
-        return;
-    }
-    // the sequence whose tokens hold t, and the token's row in its cache
-    uint32_t lo = 0, hi = p.batch;
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (p.q_begin[mid] <= t) lo = mid;
-        else hi = mid;
-    }
-    const uint32_t behind = p.q_begin[lo + 1] - t, len = p.kv_lens[lo];
-    uint32_t page = 0xFFFFFFFFu, row = 0;
-    if (t < p.q_begin[lo + 1] && behind <= len && (len - behind) / p.page_size < p.pt_stride) {
-        row = len - behind;
-        page = p.page_table[(size_t)lo * p.pt_stride + row / p.page_size];
-        row %= p.page_size;
-    }
-    if (page >= p.n_pages) {
-        if (lane == 0) atomicOr(p.status, kStatusBadPage);
-        return;
-    }
-    const size_t run = ((size_t)page * p.n_kv_heads + head) * p.page_size;  // first row of the (page, kv head) run
-    if (!K8) {
-        __half *dst = static_cast<__half *>(is_v ? p.v_pool : p.k_pool) + (run + row) * D;
-#pragma unroll
-        for (uint32_t i = 0; i < 2; ++i)
-            if (lane + 32 * i < half) {
-                dst[dim(lane + 32 * i, 0)] = a[i][0];
-                dst[dim(lane + 32 * i, 1)] = a[i][1];
-            }
-        return;
-    }
     float amax = 0.f;
 #pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) amax = fmaxf(amax, fmaxf(fabsf(__half2float(a[i][0])), fabsf(__half2float(a[i][1]))));
+    for (uint32_t e = 0; e < 8; ++e) amax = fmaxf(amax, fmaxf(fabsf(__half2float(a.h[e])), fabsf(__half2float(c.h[e]))));
+    if (!live) amax = 0.f;
 #pragma unroll
-    for (uint32_t o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const float scale = amax > 0.f ? __fdiv_rn(amax, 448.f) : 1.f;
-    uint8_t *dst = static_cast<uint8_t *>(is_v ? p.v_pool : p.k_pool) + run * D;
+    for (uint32_t o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    return amax > 0.f ? __fdiv_rn(amax, 448.f) : 1.f;
+}
+__device__ __forceinline__ uint2 bytes_of(const Chunk &x, float scale)
+{
+    union {
+        uint2 u;
+        uint8_t b[8];
+    } r;
 #pragma unroll
-    for (uint32_t i = 0; i < 2; ++i)
+    for (uint32_t e = 0; e < 8; ++e) r.b[e] = (uint8_t)__nv_cvt_float_to_fp8(__fdiv_rn(__half2float(x.h[e]), scale), __NV_SATFINITE, __NV_E4M3);
+    return r.u;
+}
+
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kInFlight = 4;   // chunk pairs a thread has in flight
+constexpr uint32_t kVHeads = 8;     // 8-bit V: kv heads transposed at a time
+
+// First block index of sequence b.  The tokens [q_begin[b], q_begin[b + 1]) touch at most (their number) / R + 2 aligned
+// blocks of R cache rows, and these starts are at least that far apart, whatever the lengths are.
+__host__ __device__ __forceinline__ uint64_t first_block(uint64_t begin, uint32_t b, uint32_t rows) { return begin / rows + 3ull * b; }
+
+template <bool K8>
+__global__ void __launch_bounds__(kThreads) mrope_append_kernel(const __grid_constant__ MropeParams p)
+{
+    constexpr uint32_t R = K8 ? 16 : 8;
+    __shared__ __align__(16) __half cos_s[R * 64], sin_s[R * 64];
+    __shared__ __align__(16) uint8_t v_s[K8 ? kVHeads * 128 * 16 : 16];
+    const uint32_t tid = threadIdx.x, D = p.head_dim, half = D / 2;
+    // The sequence whose blocks hold this one: the last whose first block is not behind it.  All threads look at once (a
+    // binary search would be a chain of loads, most of a decode step's launch).
+    uint32_t lo = 0;
+    for (uint32_t b0 = 0; b0 < p.batch; b0 += kThreads) {
+        const uint32_t b = b0 + tid;
+        const int n = __syncthreads_count(b < p.batch && first_block(__ldg(p.q_begin + b), b, R) <= blockIdx.x);
+        lo += n;
+        if (n < (int)kThreads) break;
+    }
+    lo = lo ? lo - 1 : 0;
+    const uint32_t begin = __ldg(p.q_begin + lo), end = min(__ldg(p.q_begin + lo + 1), p.tokens), len = __ldg(p.kv_lens + lo);
+    if (begin >= end) return;
+    const uint32_t n_new = end - begin, which = blockIdx.x - (uint32_t)first_block(begin, lo, R);
+    // Cache rows of this block's tokens.  A sequence shorter than its new tokens has no row for them: they are reported,
+    // their q is turned all the same (row numbers count from there).
+    const bool has_rows = n_new <= len;
+    const uint32_t start = has_rows ? len - n_new : 0, row0 = (start / R + which) * R;
+    const uint32_t first = max(row0, start), last = min(row0 + R, start + n_new);  // rows [first, last)
+    if (first >= last) return;
+    const uint32_t n_tok = last - first, t0 = begin + (first - start);
+    size_t run = 0;  // row `first` of kv head 0 in its page
+    uint32_t in_page = 0;
+    bool store = has_rows && first / p.page_size < p.pt_stride;
+    if (store) {
+        const uint32_t page = __ldg(p.page_table + (size_t)lo * p.pt_stride + first / p.page_size);
+        in_page = first % p.page_size;
+        run = (size_t)page * p.n_kv_heads * p.page_size + in_page;
+        store = page < p.n_pages;
+    }
+    if (!store && tid == 0) atomicOr(p.status, kStatusBadPage);
+
+    const uint32_t cpr = D / 16, q_slots = p.q_rot ? p.n_heads : 0;
+    const uint32_t slots = q_slots + (K8 ? p.n_kv_heads : 2 * p.n_kv_heads);  // 8-bit V rows take their own way below
+    const uint32_t total = n_tok * slots * cpr;
+    Chunk a[kInFlight], c[kInFlight];
+    auto fetch = [&](uint32_t x0) {
 #pragma unroll
-        for (uint32_t s = 0; s < 2; ++s) {
-            const uint32_t d = dim(lane + 32 * i, s);
-            dst[is_v ? v_block_offset(row, d) : row * D + d] =
-                (uint8_t)__nv_cvt_float_to_fp8(__fdiv_rn(__half2float(a[i][s]), scale), __NV_SATFINITE, __NV_E4M3);
+        for (uint32_t u = 0; u < kInFlight; ++u) {
+            const uint32_t x = x0 + u * kThreads;
+            if (x >= total) continue;
+            const uint32_t j = x % cpr, y = x / cpr, tok = y / slots, slot = y - tok * slots;
+            const uint64_t t = t0 + tok;
+            const __half *src = slot < q_slots ? p.q + t * p.q_stride + slot * D
+                                : slot < q_slots + p.n_kv_heads ? p.k + t * p.k_stride + (slot - q_slots) * D
+                                                                : p.v + t * p.v_stride + (slot - q_slots - p.n_kv_heads) * D;
+            a[u].u = __ldcs(reinterpret_cast<const uint4 *>(src + 8 * j));
+            c[u].u = __ldcs(reinterpret_cast<const uint4 *>(src + 8 * j + half));
         }
-    if (lane == 0) (is_v ? p.v_scales : p.k_scales)[run + row] = scale;
+    };
+    fetch(tid);  // on their way while the tables are gathered
+    for (uint32_t x = tid; x < n_tok * half; x += kThreads) {
+        const uint32_t tok = x / half, j = x - tok * half;
+        const uint32_t row = __ldg(p.positions + (size_t)p.axis[j] * p.pos_stride + t0 + tok);
+        __half cv = __float2half_rn(1.f), sv = __float2half_rn(0.f);
+        if (row < p.table_rows) {
+            cv = p.cos_t[(size_t)row * half + j];
+            sv = p.sin_t[(size_t)row * half + j];
+        } else {
+            atomicOr(p.status, kStatusBadPage);  // left as it is
+        }
+        cos_s[tok * half + j] = cv;
+        sin_s[tok * half + j] = sv;
+    }
+    __syncthreads();
+    for (uint32_t x0 = tid; x0 - tid < total; x0 += kInFlight * kThreads) {
+        if (x0 != tid) fetch(x0);
+#pragma unroll
+        for (uint32_t u = 0; u < kInFlight; ++u) {
+            const uint32_t x = x0 + u * kThreads;
+            const bool live = x < total;
+            if (!K8 && !live) continue;
+            const uint32_t j = x % cpr, y = x / cpr, tok = y / slots, slot = y - tok * slots;
+            const bool is_q = slot < q_slots, is_v = slot >= q_slots + p.n_kv_heads;
+            if (live && !is_v) rope_chunks(a[u], c[u], cos_s + tok * half, sin_s + tok * half, j, D, p.rope_mode);
+            if (live && is_q) {
+                __half *dst = p.q_rot + (t0 + (uint64_t)tok) * p.q_rot_stride + slot * D;
+                *reinterpret_cast<uint4 *>(dst + 8 * j) = a[u].u;
+                *reinterpret_cast<uint4 *>(dst + 8 * j + half) = c[u].u;
+            }
+            const uint32_t head = is_v ? slot - q_slots - p.n_kv_heads : slot - q_slots;
+            if (!K8) {
+                if (!is_q && store) {
+                    __half *dst = static_cast<__half *>(is_v ? p.v_pool : p.k_pool) + (run + (size_t)head * p.page_size + tok) * D;
+                    *reinterpret_cast<uint4 *>(dst + 8 * j) = a[u].u;
+                    *reinterpret_cast<uint4 *>(dst + 8 * j + half) = c[u].u;
+                }
+            } else {
+                // the eight threads of a row sit side by side
+                const float scale = row_scale(a[u], c[u], live);
+                if (live && !is_q && store) {
+                    uint8_t *dst = static_cast<uint8_t *>(p.k_pool) + (run + (size_t)head * p.page_size + tok) * 128;
+                    *reinterpret_cast<uint2 *>(dst + 8 * j) = bytes_of(a[u], scale);
+                    *reinterpret_cast<uint2 *>(dst + 8 * j + 64) = bytes_of(c[u], scale);
+                    if (j == 0) p.k_scales[run + (size_t)head * p.page_size + tok] = scale;
+                }
+            }
+        }
+    }
+    if constexpr (K8) {
+        if (!store) return;
+        // 8-bit V: [kv head][dim][16 rows of the block]
+        for (uint32_t h0 = 0; h0 < p.n_kv_heads; h0 += kVHeads) {
+            const uint32_t heads = min(kVHeads, p.n_kv_heads - h0), pairs = n_tok * heads * 8;
+            if (h0) __syncthreads();
+            for (uint32_t x0 = 0; x0 < pairs; x0 += kThreads) {
+                const uint32_t x = x0 + tid;
+                const bool live = x < pairs;
+                const uint32_t j = x % 8, head = x / 8 % heads, tok = x / 8 / heads;
+                Chunk va, vc;
+                va.u = vc.u = make_uint4(0, 0, 0, 0);
+                if (live) {
+                    const __half *src = p.v + (t0 + (uint64_t)tok) * p.v_stride + (h0 + head) * 128;
+                    va.u = __ldcs(reinterpret_cast<const uint4 *>(src + 8 * j));
+                    vc.u = __ldcs(reinterpret_cast<const uint4 *>(src + 8 * j + 64));
+                }
+                const float scale = row_scale(va, vc, live);
+                if (!live) continue;
+                union {
+                    uint2 u[2];
+                    uint8_t b[16];
+                } by;
+                by.u[0] = bytes_of(va, scale);
+                by.u[1] = bytes_of(vc, scale);
+    #pragma unroll
+                for (uint32_t e = 0; e < 16; ++e) v_s[(head * 128 + (e / 8) * 64 + 8 * j + e % 8) * 16 + tok] = by.b[e];
+                if (j == 0) p.v_scales[run + (size_t)(h0 + head) * p.page_size + tok] = scale;
+            }
+            __syncthreads();
+            const uint32_t r = in_page % 16;  // row of the block that token 0 goes to (0 where the block is whole)
+            for (uint32_t x = tid; x < heads * 128; x += kThreads) {
+                const uint32_t head = x / 128, d = x % 128;
+                uint8_t *dst = static_cast<uint8_t *>(p.v_pool) + (run - in_page + (size_t)(h0 + head) * p.page_size) * 128 + in_page / 16 * 2048 + d * 16 + r;
+                if (n_tok == 16) *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(v_s + x * 16);
+                else
+                    for (uint32_t t = 0; t < n_tok; ++t) dst[t] = v_s[x * 16 + t];
+            }
+        }
+    }
 }
 
 template <class Cache>
@@ -182,10 +266,10 @@ template <bool K8>
 mf_status launch_mrope(MfContext *ctx, const MropeParams &p, const char *what)
 {
     if (p.tokens == 0) return MF_OK;
-    const uint64_t warps = (uint64_t)p.tokens * ((p.q_rot ? p.n_heads : 0) + 2 * (uint64_t)p.n_kv_heads);
-    if ((warps + 7) / 8 > 0x7FFFFFFFull) return fail(ctx, MF_ERR_INVALID_SHAPE, "%s: %u tokens", what, p.tokens);
+    const uint64_t blocks = first_block(p.tokens, p.batch, K8 ? 16 : 8) + 1;
+    if (blocks > 0x7FFFFFFFull) return fail(ctx, MF_ERR_INVALID_SHAPE, "%s: %u tokens of %u sequences", what, p.tokens, p.batch);
     DeviceScope scope(ctx->device);
-    mrope_append_kernel<K8><<<(uint32_t)((warps + 7) / 8), 256, 0, ctx->stream>>>(p);
+    mrope_append_kernel<K8><<<(uint32_t)blocks, kThreads, 0, ctx->stream>>>(p);
     return check_launch(ctx, "mrope_append_kernel");
 }
 
@@ -199,6 +283,8 @@ extern "C" {
 mf_status mf_paged_mrope_append(MfContext *ctx, const MfPagedKv *c, const MfMropeAppendArgs *a)
 {
     if (!ctx) return MF_ERR_INPUT_NOT_FOUND;
+    if (c && c->page_size % 8)
+        return fail(ctx, MF_ERR_OPERATION_NOT_SUPPORTED, "mrope append: page_size %u (a multiple of 8)", c->page_size);
     if (c && (c->head_dim != 64 && c->head_dim != 128))
         return fail(ctx, MF_ERR_OPERATION_NOT_SUPPORTED, "mrope append: head_dim %u (64 or 128)", c->head_dim);
     MropeParams p{};
