@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 
 import numpy as np
 from pathlib import Path
@@ -151,6 +152,11 @@ class MfMropeAppendArgs(C.Structure):
                 ("axis", C.c_uint8 * 64)]
 
 
+# The two structs above as one pack call each: filling a ctypes structure field by field is most of a small call's time.
+_CHUNK_ARGS = struct.Struct("=6Qf4x")
+_MROPE_ARGS = struct.Struct("=12Q6I64s")
+
+
 class MfFusedQkvArgs(C.Structure):
     _fields_ = [("input", vp), ("w_q", vp), ("w_k", vp), ("w_v", vp), ("gamma", vp), ("bias_q", vp), ("bias_k", vp),
                 ("bias_v", vp), ("out_q", vp), ("out_k", vp), ("out_v", vp), ("k_dim", u32), ("n_dim", u32),
@@ -263,9 +269,9 @@ _SIGNATURES = {
     "mf_chunk_plan_destroy": (None, [vp, vp]),
     "mf_chunk_plan_tokens": (u32, [vp]),
     "mf_chunk_plan_build_host": (u32, [vp, vp] + [u32] * 7 + [vp, u32, vp]),
-    "mf_paged_chunk_attention": (C.c_int32, [vp, vp, C.POINTER(MfPagedKv), C.POINTER(MfPagedChunkArgs)]),
-    "mf_paged_mrope_append": (C.c_int32, [vp, C.POINTER(MfPagedKv), C.POINTER(MfMropeAppendArgs)]),
-    "mf_paged_kv8_mrope_append": (C.c_int32, [vp, C.POINTER(MfPagedKv8), C.POINTER(MfMropeAppendArgs)]),
+    "mf_paged_chunk_attention": (C.c_int32, [vp, vp, C.POINTER(MfPagedKv), vp]),
+    "mf_paged_mrope_append": (C.c_int32, [vp, C.POINTER(MfPagedKv), vp]),
+    "mf_paged_kv8_mrope_append": (C.c_int32, [vp, C.POINTER(MfPagedKv8), vp]),
     "mf_paged_move_pages": (C.c_int32, [vp, vp, u32, vp, vp, u32]),
     "mf_paged_kv8_move_pages": (C.c_int32, [vp, vp, u32, vp, vp, u32]),
     "mf_page_pool_fork": (C.c_int32, [vp, vp, u32, u32, vp, C.POINTER(u32), C.POINTER(u32)]),
@@ -552,8 +558,8 @@ class Foundry:
         d = cache.head_dim
         qt, qh = _head_strides(q, plan, d, "q")
         ot, oh = _head_strides(out, plan, d, "out")
-        a = MfPagedChunkArgs(q.data_ptr(), out.data_ptr(), qt, qh, ot, oh, d ** -0.5 if scale is None else scale)
-        self.check(lib.mf_paged_chunk_attention(self._h, plan._h, C.byref(cache), C.byref(a)))
+        a = _CHUNK_ARGS.pack(q.data_ptr(), out.data_ptr(), qt, qh, ot, oh, d ** -0.5 if scale is None else scale)
+        self.check(lib.mf_paged_chunk_attention(self._h, plan._h, C.byref(cache), a))
 
     def paged_mrope_append(self, cache, q, k, v, q_rot, cos, sin, positions, q_begin, axes, *, n_heads,
                            rope_mode=ROPE_MODE_NEOX):
@@ -566,7 +572,7 @@ class Foundry:
         q_stride = _row_stride(q, tokens, n_heads * d, "q") if q is not None else 0
         rot_stride = _row_stride(q_rot, tokens, n_heads * d, "q_rot") if q_rot is not None else 0
         rows = cos.shape[0]
-        if cos.shape != (rows, half) or sin.shape != (rows, half) or not (cos.is_contiguous() and sin.is_contiguous()):
+        if not (cos.numel() == rows * half == sin.numel() and cos.is_contiguous() and sin.is_contiguous()):
             raise MetalError(2, f"mrope append: cos / sin must be [rows, {half}]")
         p_strides = positions.stride()
         if len(p_strides) != 2 or positions.shape[1] != tokens or p_strides[1] != 1 or positions.element_size() != 4:
@@ -576,12 +582,11 @@ class Foundry:
         if len(axes) != half:
             raise MetalError(2, f"mrope append: {len(axes)} axes for {half} frequencies")
         n_axes = positions.shape[0]
-        a = MfMropeAppendArgs(_ptr(q), k.data_ptr(), v.data_ptr(), _ptr(q_rot), cos.data_ptr(), sin.data_ptr(),
-                              positions.data_ptr(), q_begin.data_ptr(), q_stride, k_stride, v_stride, rot_stride, tokens, n_heads,
-                              n_axes, p_strides[0] if n_axes > 1 else tokens, rows, rope_mode)
-        C.memmove(a.axis, bytes(axes), len(axes))
+        a = _MROPE_ARGS.pack(_ptr(q) or 0, k.data_ptr(), v.data_ptr(), _ptr(q_rot) or 0, cos.data_ptr(), sin.data_ptr(),
+                             positions.data_ptr(), q_begin.data_ptr(), q_stride, k_stride, v_stride, rot_stride, tokens, n_heads,
+                             n_axes, p_strides[0] if n_axes > 1 else tokens, rows, rope_mode, bytes(axes))
         fn = lib.mf_paged_kv8_mrope_append if isinstance(cache, MfPagedKv8) else lib.mf_paged_mrope_append
-        self.check(fn(self._h, C.byref(cache), C.byref(a)))
+        self.check(fn(self._h, C.byref(cache), a))
 
     def paged_move_pages(self, layers, src_ids, dst_ids):
         """Pages dst <- src in all layers (kv_layers of f16 or 8-bit caches); the ids are host arrays (numpy uint32)."""
@@ -589,7 +594,7 @@ class Foundry:
         if src.size != dst.size:
             raise MetalError(2, f"move pages: {src.size} sources, {dst.size} destinations")
         fn = lib.mf_paged_kv8_move_pages if layers._type_ is MfPagedKv8 else lib.mf_paged_move_pages
-        self.check(fn(self._h, layers, len(layers), src.ctypes.data, dst.ctypes.data, src.size))
+        self.check(fn(self._h, layers, len(layers), src.tobytes(), dst.tobytes(), src.size))
 
     def paged_kv_append(self, cache: MfPagedKv, q, k, v, q_rot, cos, sin, *, n_heads, rope_mode=ROPE_MODE_NEOX,
                         apply_rope=True, seq=ALL_SEQUENCES, position_offset=0, seq_len=0):
@@ -917,8 +922,10 @@ def _head_strides(x, plan: ChunkPlan, d: int, name: str):
 
 def _row_stride(x, rows: int, cols: int, name: str) -> int:
     """Row stride of f16 [rows, cols] with unit column stride."""
+    if x.numel() == rows * cols and x.is_contiguous() and x.element_size() == 2 and x.dim() == 2:
+        return cols
     st = x.stride()
-    if x.shape != (rows, cols) or st[1] != 1 or x.element_size() != 2:
+    if x.shape != (rows, cols) or st[-1] != 1 or x.element_size() != 2:
         raise MetalError(2, f"mrope append: {name} must be f16 [{rows}, {cols}] with unit column stride")
     return st[0]
 

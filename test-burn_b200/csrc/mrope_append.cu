@@ -11,6 +11,8 @@
 // whole block goes out as 16-byte words, a part of one byte by byte.
 #include <cuda_fp8.h>
 
+#include <algorithm>
+
 #include "append.cuh"
 #include "internal.hpp"
 
@@ -27,6 +29,7 @@ struct MropeParams {
     uint32_t *status;
     uint64_t q_stride, k_stride, v_stride, q_rot_stride;
     uint32_t tokens, batch, n_heads, n_kv_heads, head_dim, page_size, pt_stride, n_pages, pos_stride, table_rows, rope_mode;
+    uint32_t slots_per_part;  // head slots a CTA takes
     uint8_t axis[64];
 };
 
@@ -53,31 +56,33 @@ __device__ __forceinline__ uint2 bytes_of(const Chunk &x, float scale)
 }
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kInFlight = 4;   // chunk pairs a thread has in flight
+__host__ __device__ constexpr uint32_t in_flight(bool k8) { return k8 ? 2 : 4; }  // chunk pairs a thread has in flight
 constexpr uint32_t kVHeads = 8;     // 8-bit V: kv heads transposed at a time
 
 // First block index of sequence b.  The tokens [q_begin[b], q_begin[b + 1]) touch at most (their number) / R + 2 aligned
 // blocks of R cache rows, and these starts are at least that far apart, whatever the lengths are.
 __host__ __device__ __forceinline__ uint64_t first_block(uint64_t begin, uint32_t b, uint32_t rows) { return begin / rows + 3ull * b; }
 
-template <bool K8>
-__global__ void __launch_bounds__(kThreads) mrope_append_kernel(const __grid_constant__ MropeParams p)
+// blockIdx: (block of rows, part of the head slots); the last part of the 8-bit form has the V rows.
+template <uint32_t D, bool K8>
+__global__ void __launch_bounds__(kThreads, 4) mrope_append_kernel(const __grid_constant__ MropeParams p)
 {
-    constexpr uint32_t R = K8 ? 16 : 8;
-    __shared__ __align__(16) __half cos_s[R * 64], sin_s[R * 64];
+    constexpr uint32_t R = K8 ? 16 : 8, half = D / 2, cpr = D / 16;  // cpr: chunk pairs per head row
+    __shared__ __align__(16) __half cos_s[R * half], sin_s[R * half];
+    __shared__ uint4 found_s;  // sequence, its tokens [y, z), its length
     __shared__ __align__(16) uint8_t v_s[K8 ? kVHeads * 128 * 16 : 16];
-    const uint32_t tid = threadIdx.x, D = p.head_dim, half = D / 2;
-    // The sequence whose blocks hold this one: the last whose first block is not behind it.  All threads look at once (a
-    // binary search would be a chain of loads, most of a decode step's launch).
-    uint32_t lo = 0;
-    for (uint32_t b0 = 0; b0 < p.batch; b0 += kThreads) {
-        const uint32_t b = b0 + tid;
-        const int n = __syncthreads_count(b < p.batch && first_block(__ldg(p.q_begin + b), b, R) <= blockIdx.x);
-        lo += n;
-        if (n < (int)kThreads) break;
+    const uint32_t tid = threadIdx.x;
+    // The sequence whose blocks hold this one, found by the thread that looks at it (a binary search would be a chain of
+    // loads, most of a decode step's launch).
+    if (tid == 0) found_s = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    for (uint32_t b = tid; b < p.batch; b += kThreads) {
+        const uint32_t b0 = __ldg(p.q_begin + b), b1 = min(__ldg(p.q_begin + b + 1), p.tokens), kv = __ldg(p.kv_lens + b);
+        const uint64_t mine = first_block(b0, b, R);
+        if (b0 < b1 && mine <= blockIdx.x && blockIdx.x - mine <= (b1 - b0) / R + 1) found_s = make_uint4(b, b0, b1, kv);
     }
-    lo = lo ? lo - 1 : 0;
-    const uint32_t begin = __ldg(p.q_begin + lo), end = min(__ldg(p.q_begin + lo + 1), p.tokens), len = __ldg(p.kv_lens + lo);
+    __syncthreads();
+    const uint32_t lo = found_s.x, begin = found_s.y, end = found_s.z, len = found_s.w;
     if (begin >= end) return;
     const uint32_t n_new = end - begin, which = blockIdx.x - (uint32_t)first_block(begin, lo, R);
     // Cache rows of this block's tokens.  A sequence shorter than its new tokens has no row for them: they are reported,
@@ -87,28 +92,34 @@ __global__ void __launch_bounds__(kThreads) mrope_append_kernel(const __grid_con
     const uint32_t first = max(row0, start), last = min(row0 + R, start + n_new);  // rows [first, last)
     if (first >= last) return;
     const uint32_t n_tok = last - first, t0 = begin + (first - start);
-    size_t run = 0;  // row `first` of kv head 0 in its page
-    uint32_t in_page = 0;
-    bool store = has_rows && first / p.page_size < p.pt_stride;
-    if (store) {
-        const uint32_t page = __ldg(p.page_table + (size_t)lo * p.pt_stride + first / p.page_size);
-        in_page = first % p.page_size;
-        run = (size_t)page * p.n_kv_heads * p.page_size + in_page;
-        store = page < p.n_pages;
-    }
-    if (!store && tid == 0) atomicOr(p.status, kStatusBadPage);
-
-    const uint32_t cpr = D / 16, q_slots = p.q_rot ? p.n_heads : 0;
+    const bool in_table = has_rows && first / p.page_size < p.pt_stride;
+    const uint32_t page = in_table ? __ldg(p.page_table + (size_t)lo * p.pt_stride + first / p.page_size) : 0xFFFFFFFFu;
+    const uint32_t in_page = first % p.page_size;
+    const uint32_t q_slots = p.q_rot ? p.n_heads : 0;
     const uint32_t slots = q_slots + (K8 ? p.n_kv_heads : 2 * p.n_kv_heads);  // 8-bit V rows take their own way below
-    const uint32_t total = n_tok * slots * cpr;
+    const uint32_t part0 = blockIdx.y * p.slots_per_part, width = part0 < slots ? min(p.slots_per_part, slots - part0) : 0;
+    // Pair x of the part: chunk j = x % cpr of slot part0 + (x / cpr) % width of token x / cpr / width.  A thread's pairs
+    // are kThreads apart: j stays, (token, slot) advance without a division.
+    const uint32_t j = tid % cpr, rows = n_tok * width;
+    struct At {
+        uint32_t row, tok, slot;
+    };
+    auto advance = [&](At &at) {
+        at.row += kThreads / cpr;
+        at.slot += kThreads / cpr;
+        while (at.slot >= width && at.row < rows) at.slot -= width, ++at.tok;
+    };
+    At in{tid / cpr, 0, tid / cpr};
+    while (in.slot >= width && in.row < rows) in.slot -= width, ++in.tok;
+    At out = in;
+    constexpr uint32_t kInFlight = in_flight(K8);
     Chunk a[kInFlight], c[kInFlight];
-    auto fetch = [&](uint32_t x0) {
+    auto fetch = [&]() {
 #pragma unroll
-        for (uint32_t u = 0; u < kInFlight; ++u) {
-            const uint32_t x = x0 + u * kThreads;
-            if (x >= total) continue;
-            const uint32_t j = x % cpr, y = x / cpr, tok = y / slots, slot = y - tok * slots;
-            const uint64_t t = t0 + tok;
+        for (uint32_t u = 0; u < kInFlight; ++u, advance(in)) {
+            if (in.row >= rows) continue;
+            const uint64_t t = t0 + in.tok;
+            const uint32_t slot = part0 + in.slot;
             const __half *src = slot < q_slots ? p.q + t * p.q_stride + slot * D
                                 : slot < q_slots + p.n_kv_heads ? p.k + t * p.k_stride + (slot - q_slots) * D
                                                                 : p.v + t * p.v_stride + (slot - q_slots - p.n_kv_heads) * D;
@@ -116,8 +127,8 @@ __global__ void __launch_bounds__(kThreads) mrope_append_kernel(const __grid_con
             c[u].u = __ldcs(reinterpret_cast<const uint4 *>(src + 8 * j + half));
         }
     };
-    fetch(tid);  // on their way while the tables are gathered
-    for (uint32_t x = tid; x < n_tok * half; x += kThreads) {
+    fetch();  // on their way while the tables are gathered
+    for (uint32_t x = tid; x < (width ? n_tok * half : 0); x += kThreads) {
         const uint32_t tok = x / half, j = x - tok * half;
         const uint32_t row = __ldg(p.positions + (size_t)p.axis[j] * p.pos_stride + t0 + tok);
         __half cv = __float2half_rn(1.f), sv = __float2half_rn(0.f);
@@ -130,15 +141,17 @@ __global__ void __launch_bounds__(kThreads) mrope_append_kernel(const __grid_con
         cos_s[tok * half + j] = cv;
         sin_s[tok * half + j] = sv;
     }
+    const bool store = page < p.n_pages;
+    const size_t run = (size_t)page * p.n_kv_heads * p.page_size + in_page;  // row `first` of kv head 0 in its page
+    if (!store && tid == 0) atomicOr(p.status, kStatusBadPage);
     __syncthreads();
-    for (uint32_t x0 = tid; x0 - tid < total; x0 += kInFlight * kThreads) {
-        if (x0 != tid) fetch(x0);
+    for (uint32_t r0 = 0; r0 < rows; r0 += kInFlight * (kThreads / cpr)) {
+        if (r0) fetch();
 #pragma unroll
-        for (uint32_t u = 0; u < kInFlight; ++u) {
-            const uint32_t x = x0 + u * kThreads;
-            const bool live = x < total;
+        for (uint32_t u = 0; u < kInFlight; ++u, advance(out)) {
+            const bool live = out.row < rows;
             if (!K8 && !live) continue;
-            const uint32_t j = x % cpr, y = x / cpr, tok = y / slots, slot = y - tok * slots;
+            const uint32_t tok = out.tok, slot = part0 + out.slot;
             const bool is_q = slot < q_slots, is_v = slot >= q_slots + p.n_kv_heads;
             if (live && !is_v) rope_chunks(a[u], c[u], cos_s + tok * half, sin_s + tok * half, j, D, p.rope_mode);
             if (live && is_q) {
@@ -155,6 +168,7 @@ __global__ void __launch_bounds__(kThreads) mrope_append_kernel(const __grid_con
                 }
             } else {
                 // the eight threads of a row sit side by side
+                if (!__any_sync(0xffffffffu, live && !is_q)) continue;
                 const float scale = row_scale(a[u], c[u], live);
                 if (live && !is_q && store) {
                     uint8_t *dst = static_cast<uint8_t *>(p.k_pool) + (run + (size_t)head * p.page_size + tok) * 128;
@@ -166,7 +180,7 @@ __global__ void __launch_bounds__(kThreads) mrope_append_kernel(const __grid_con
         }
     }
     if constexpr (K8) {
-        if (!store) return;
+        if (!store || width) return;
         // 8-bit V: [kv head][dim][16 rows of the block]
         for (uint32_t h0 = 0; h0 < p.n_kv_heads; h0 += kVHeads) {
             const uint32_t heads = min(kVHeads, p.n_kv_heads - h0), pairs = n_tok * heads * 8;
@@ -263,13 +277,23 @@ mf_status mrope_params(MfContext *ctx, const Cache *c, const MfMropeAppendArgs *
 }
 
 template <bool K8>
-mf_status launch_mrope(MfContext *ctx, const MropeParams &p, const char *what)
+mf_status launch_mrope(MfContext *ctx, MropeParams &p, const char *what)
 {
     if (p.tokens == 0) return MF_OK;
-    const uint64_t blocks = first_block(p.tokens, p.batch, K8 ? 16 : 8) + 1;
+    const uint32_t R = K8 ? 16 : 8, cpr = p.head_dim / 16;
+    const uint64_t blocks = first_block(p.tokens, p.batch, R) + 1;
+    const uint64_t slots = (p.q_rot ? p.n_heads : 0) + (uint64_t)(K8 ? 1 : 2) * p.n_kv_heads;
+    // Prompts: so many parts that a whole block leaves every thread one round of loads.  Decode steps (a token or few per
+    // sequence) have little for a CTA as it is.
+    uint64_t parts = 1;
+    if (p.tokens >= 4ull * p.batch) parts = std::min<uint64_t>((R * slots * cpr + in_flight(K8) * kThreads - 1) / (in_flight(K8) * kThreads), 64);
+    p.slots_per_part = (uint32_t)((slots + parts - 1) / parts);
+    parts = (slots + p.slots_per_part - 1) / p.slots_per_part + (K8 ? 1 : 0);
     if (blocks > 0x7FFFFFFFull) return fail(ctx, MF_ERR_INVALID_SHAPE, "%s: %u tokens of %u sequences", what, p.tokens, p.batch);
     DeviceScope scope(ctx->device);
-    mrope_append_kernel<K8><<<(uint32_t)blocks, kThreads, 0, ctx->stream>>>(p);
+    const dim3 grid((uint32_t)blocks, (uint32_t)parts);
+    if (p.head_dim == 128) mrope_append_kernel<128, K8><<<grid, kThreads, 0, ctx->stream>>>(p);
+    else if constexpr (!K8) mrope_append_kernel<64, false><<<grid, kThreads, 0, ctx->stream>>>(p);
     return check_launch(ctx, "mrope_append_kernel");
 }
 
