@@ -11,11 +11,12 @@
 //   more than 128 rows   the streams are the two query tiles, both work on every key tile ("paired rows")
 //   up to 128 rows       both streams hold the same rows, stream s takes the key tiles s, s + 2, ... and the two states
 //                        are merged when the item ends ("paired keys"): decode and short chunks
-// A stream is one chain  S = Q K^T -> max, exp, P (f16, over S) -> O += P V -> next tile;  while its softmax group
-// works, the tensor pipe works for the other stream.  Nothing is handed from one group to the other between tiles.
+// A stream takes its key tiles in two halves of 64 keys, each with score columns of its own: S = Q K^T -> max, exp, P (f16,
+// over S) -> O += P V -> the same half of the next tile.  While a softmax group works on one half, the tensor pipe has
+// the other half and the other stream; a group waits for nothing but its own two halves.
 //
 //   warps 0-3, 4-7  softmax groups (one thread per row = TMEM lane)   warp 8   TMA producer, one copy per page and tile
-//   warp 9          issues the products                               warp 10  loads q, allocates TMEM
+//   warps 9, 10     issue the products of streams 0, 1                warp 11  loads q, allocates TMEM
 //
 // K and V tiles share one ring in the order in which the products want them.  A (page, kv head) run lands as
 // [8-row group][half][8 rows][128 bytes], so the 128 rows of a tile are evenly spaced 8-row groups whatever the page
@@ -29,7 +30,7 @@
 // others when it is not finite; then the output is not finite either, and such a row is walked again key by key
 // (walk_row).
 //
-// TMEM columns (512): S_0/P_0 [0,128)  S_1/P_1 [128,256)  O_0 [256,384)  O_1 [384,512).
+// TMEM columns (512): halves 0, 1 of S_0/P_0 [0,64) [64,128), of S_1/P_1 [128,192) [192,256), O_0 [256,384)  O_1 [384,512).
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -66,8 +67,8 @@ namespace {
 constexpr uint32_t kMaxGroup = 64;
 constexpr uint32_t kMaxLen = 1u << 30;  // positions and tile arithmetic stay inside 32 bits
 constexpr uint32_t kTile = kChunkTile;
-constexpr uint32_t kThreads = 352;
-constexpr uint32_t kProducerWarp = 8, kIssuerWarp = 9, kQWarp = 10;
+constexpr uint32_t kThreads = 384;
+constexpr uint32_t kProducerWarp = 8, kIssuerWarp = 9, kQWarp = 11;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr float kNegInf = -1e30f;
 constexpr float kRescaleThreshold = 8.0f;  // log2 of the largest weight kept in P
@@ -76,13 +77,14 @@ constexpr uint32_t kHalfTile = kTile * 128;
 __host__ __device__ constexpr uint32_t tile_bytes(uint32_t d) { return kTile * d * 2; }
 __host__ __device__ constexpr uint32_t ring_slots(uint32_t d) { return d == 128 ? 5 : 10; }
 enum Bar : uint32_t {
-    kSFull = 0,   // [2] scores of the stream's next tile are in S (and its last P V has completed)
-    kPFull = 2,   // [2] weights are in P, O has been rescaled if needed
-    kOFull = 4,   // [2] the item's last P V has completed
-    kOFree = 6,   // [2] the item's O has been read (8 arrivals)
-    kQFull = 8,
-    kQFree = 9,   // the item's last Q K^T has completed
-    kFull = 10    // [slots], then empty [slots]
+    kSFull = 0,   // [stream * 2 + half] scores of the next tile's half are in S
+    kPFull = 4,   // [stream * 2 + half] weights are in P, O has been rescaled if needed
+    kODone = 8,   // [stream] a P V has completed (one phase per half tile)
+    kOFull = 10,  // [stream] the item's last P V has completed
+    kOFree = 12,  // [stream] the item's O has been read (8 arrivals)
+    kQFull = 14,
+    kQFree = 15,  // 2 arrivals: the streams' last Q K^T of the item
+    kFull = 16    // [slots], then empty [slots] (2 arrivals: the streams)
 };
 __host__ __device__ constexpr uint32_t num_bars(uint32_t d) { return kFull + 2 * ring_slots(d); }
 constexpr uint32_t kMlBytes = 2 * kTile * 8;  // (m, l) of the two streams' rows
@@ -199,7 +201,9 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     volatile uint32_t *words = reinterpret_cast<volatile uint32_t *>(smem + kBytes * (2 + kSlots) + kMlBytes + num_bars(D) * 8);
     volatile uint32_t *abort_flag = words + 1;
     auto bar = [&](uint32_t i) { return bars + i * 8; };
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // (the warp's number by a shuffle: known to be the same in all its lanes, so that what the issuing warp computes stays
+    // in uniform registers)
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t G = p.group, half_tok = kTile / G;
     const uint32_t item0 = __ldg(p.list + blockIdx.x), item1 = __ldg(p.list + blockIdx.x + 1);
     if (item0 >= item1) return;
@@ -208,17 +212,20 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         return;
     }
     if (tid == 0) {
-        for (uint32_t s = 0; s < 2; ++s) {
+        for (uint32_t s = 0; s < 4; ++s) {
             mbar_init(bar(kSFull + s), 1);
             mbar_init(bar(kPFull + s), 4);
+        }
+        for (uint32_t s = 0; s < 2; ++s) {
+            mbar_init(bar(kODone + s), 1);
             mbar_init(bar(kOFull + s), 1);
             mbar_init(bar(kOFree + s), 8);
         }
         mbar_init(bar(kQFull), 1);
-        mbar_init(bar(kQFree), 1);
+        mbar_init(bar(kQFree), 2);
         for (uint32_t s = 0; s < kSlots; ++s) {
             mbar_init(bar(kFull + s), 1);
-            mbar_init(bar(kFull + kSlots + s), 1);
+            mbar_init(bar(kFull + kSlots + s), 2);
         }
         *abort_flag = 0;
         mbar_fence_init();
@@ -339,81 +346,91 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(kQFull));
         }
-    } else if (warp == kIssuerWarp) {
-        // ------------------------------------------------------- the products of both streams (one warp) ---
-        // The streams take turns, P V of a tile and Q K^T of the stream's next one at a time: the softmax of one then
-        // runs while the tensor pipe works for the other.  (Issued by a thread each, the two blocks share the pipe, end
-        // together and leave it idle together: 6 000 cycles per pair of tiles instead of the sum of either half.)
-        {
-            const uint32_t elected = elect_one_sync();
-            constexpr uint32_t kIdescQK = instr_desc_f16(kTile, kTile, 0), kIdescPV = instr_desc_f16(kTile, D, 1);
-            constexpr uint32_t kGroupStride = 16 * D;  // bytes between 8-row groups of a K or V tile
-            uint32_t q_phase = 0, p_phase[2] = {0, 0}, o_uses[2] = {0, 0}, loads = 0;
-            auto full = [&](uint32_t load) {
-                wait(bar(kFull + load % kSlots), (load / kSlots) & 1, 16u);
-                return ring + load % kSlots * kBytes;
+    } else if (warp >= kIssuerWarp) {
+        // -------------------------------------------------------- the products of one stream (whole warp) ---
+        // P V of a half tile and Q K^T of the same half of the stream's next tile, in turn for the two halves.  A warp per
+        // stream: what the issue of a block costs (some 1 000 cycles with its waits) is as long as the block itself, and one
+        // warp for both would be the kernel's pace.
+        const uint32_t s = warp - kIssuerWarp, elected = elect_one_sync();
+        constexpr uint32_t kIdescQK = instr_desc_f16(kTile, kTile / 2, 0), kIdescPV = instr_desc_f16(kTile, D, 1);
+        constexpr uint32_t kGroupStride = 16 * D;  // bytes between 8-row groups of a K or V tile
+        struct Place {  // of a tile in the ring
+            uint32_t slot, phase;
+        };
+        auto ahead = [&](Place at, uint32_t by) {
+            at.slot += by;
+            if (at.slot >= kSlots) at.slot -= kSlots, at.phase ^= 1;
+            return at;
+        };
+        uint32_t q_phase = 0, p_phase = 0, o_uses = 0;
+        Place base{0, 0};
+        for (uint32_t i = item0; i < item1; ++i) {
+            const ChunkItem it = load_item(p, i);
+            const uint32_t n = it.tile_end - it.tile_begin;
+            if (n == 0) continue;
+            const bool paired_rows = it.n_tok > half_tok;
+            const uint32_t tiles = paired_rows ? n : (n + 1 - s) / 2;
+            const uint64_t q_desc = smem_desc(q_smem + (paired_rows ? s * kBytes : 0), 16, 1024);
+            // paired rows: K V K V ..., for both streams; paired keys: K0 K1 V0 V1 ..., a last single tile K0 V0
+            Place k = paired_rows ? base : ahead(base, s), v = k;
+            auto release = [&](uint32_t slot) {
+                tc_commit_elected(elected, bar(kFull + kSlots + slot));
+                if (!paired_rows) tc_commit_elected(elected, bar(kFull + kSlots + slot));  // for the other stream too
             };
-            auto release = [&](uint32_t load) { tc_commit_elected(elected, bar(kFull + kSlots + load % kSlots)); };
-            for (uint32_t i = item0; i < item1; ++i) {
-                const ChunkItem it = load_item(p, i);
-                const uint32_t n = it.tile_end - it.tile_begin;
-                if (n == 0) continue;
-                const bool paired_rows = it.n_tok > half_tok;
-                const uint32_t tiles[2] = {paired_rows ? n : (n + 1) / 2, paired_rows ? n : n / 2};
-                auto scores = [&](uint32_t s, uint32_t j) {
-                    const uint32_t load = loads + (paired_rows ? 2 * j : 4 * j + s);
-                    const uint64_t k_desc = smem_desc(full(load), 16, kGroupStride);
-                    const uint64_t q_desc = smem_desc(q_smem + (paired_rows ? s * kBytes : 0), 16, 1024);
+            auto scores = [&](uint32_t h) {
+                wait(bar(kFull + k.slot), k.phase, 16u);
+                const uint64_t k_desc = smem_desc(ring + k.slot * kBytes + h * 8 * kGroupStride, 16, kGroupStride);
+                tc_fence_after();
+#pragma unroll
+                for (uint32_t kk = 0; kk < D / 16; ++kk)
+                    tc_mma_ss_elected(elected, tmem + s * 128 + h * 64, q_desc + (((kk >> 2) * kHalfTile + (kk & 3) * 32) >> 4),
+                                      k_desc + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4), kIdescQK, kk > 0);
+                tc_commit_elected(elected, bar(kSFull + s * 2 + h));
+                if (h == 1) release(k.slot);
+            };
+            wait(bar(kQFull), q_phase, 32u);
+            q_phase ^= 1;
+            if (tiles) {
+                scores(0);
+                scores(1);
+            }
+            if (tiles <= 1) tc_commit_elected(elected, bar(kQFree));
+            for (uint32_t j = 0; j < tiles; ++j) {
+                const bool more = j + 1 < tiles;
+                v = ahead(k, paired_rows || 2 * j + 1 >= n ? 1 : 2);
+                if (more) k = ahead(k, paired_rows ? 2 : 4);
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    if (h == 0) wait(bar(kFull + v.slot), v.phase, 16u);
+                    const uint64_t v_desc = smem_desc(ring + v.slot * kBytes + h * 8 * kGroupStride, 1024, kGroupStride);
+                    wait(bar(kPFull + s * 2 + h), p_phase, 64u);
+                    if (j == 0 && h == 0 && o_uses) wait(bar(kOFree + s), (o_uses - 1) & 1, 128u);
                     tc_fence_after();
 #pragma unroll
-                    for (uint32_t kk = 0; kk < D / 16; ++kk)
-                        tc_mma_ss_elected(elected, tmem + s * 128, q_desc + (((kk >> 2) * kHalfTile + (kk & 3) * 32) >> 4),
-                                  k_desc + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4), kIdescQK, kk > 0);
-                    tc_commit_elected(elected, bar(kSFull + s));
-                    if (!paired_rows || s == 1) release(load);
-                };
-                wait(bar(kQFull), q_phase, 32u);
-                q_phase ^= 1;
-                scores(0, 0);
-                if (tiles[1]) scores(1, 0);
-                if (tiles[0] == 1) tc_commit_elected(elected, bar(kQFree));
-                for (uint32_t j = 0; j < tiles[0]; ++j)
-#pragma unroll
-                    for (uint32_t s = 0; s < 2; ++s) {
-                        if (j >= tiles[s]) continue;
-                        const uint32_t load = loads + (paired_rows ? 2 * j + 1 : 4 * j + (2 * j + 1 < n ? 2 + s : 1));
-                        const uint64_t v_desc = smem_desc(full(load), 1024, kGroupStride);
-                        wait(bar(kPFull + s), p_phase[s], 64u);
-                        p_phase[s] ^= 1;
-                        if (j == 0 && o_uses[s]) wait(bar(kOFree + s), (o_uses[s] - 1) & 1, 128u);
-                        tc_fence_after();
-#pragma unroll
-                        for (uint32_t kk = 0; kk < kTile / 16; ++kk)
-                            tc_mma_ts_elected(elected, tmem + 256 + s * 128, tmem + s * 128 + kk * 8, v_desc + ((kk * 2 * kGroupStride) >> 4), kIdescPV,
-                                      (j > 0 || kk > 0) ? 1u : 0u);
-                        if (!paired_rows || s == 1) release(load);
-                        if (j + 1 == tiles[s]) {
-                            tc_commit_elected(elected, bar(kOFull + s));
-                        } else {
-                            scores(s, j + 1);
-                            // the last Q K^T of the item: stream 1's where it has as many tiles
-                            if (j + 2 == tiles[0] && s == (tiles[1] == tiles[0] ? 1u : 0u)) tc_commit_elected(elected, bar(kQFree));
-                        }
-                    }
-                ++o_uses[0];
-                o_uses[1] += tiles[1] > 0;
-                loads += 2 * n;
+                    for (uint32_t kk = 0; kk < kTile / 32; ++kk)
+                        tc_mma_ts_elected(elected, tmem + 256 + s * 128, tmem + s * 128 + h * 64 + kk * 8,
+                                          v_desc + ((kk * 2 * kGroupStride) >> 4), kIdescPV, (j > 0 || h > 0 || kk > 0) ? 1u : 0u);
+                    tc_commit_elected(elected, bar(kODone + s));
+                    if (h == 1) release(v.slot);
+                    if (more) scores(h);
+                }
+                p_phase ^= 1;
+                if (!more) tc_commit_elected(elected, bar(kOFull + s));
+                if (j + 2 == tiles) tc_commit_elected(elected, bar(kQFree));
             }
-            // The products have to be over before the TMEM goes back (they are, unless a wait ran out).
-            for (uint32_t s = 0; s < 2; ++s)
-                if (o_uses[s]) wait(bar(kOFull + s), (o_uses[s] - 1) & 1, 256u);
+            o_uses += tiles > 0;
+            const uint32_t skip = (2 * n) % kSlots;
+            base.phase ^= ((2 * n) / kSlots) & 1;
+            base = ahead(base, skip);
         }
+        // The products have to be over before the TMEM goes back (they are, unless a wait ran out).
+        if (o_uses) wait(bar(kOFull + s), (o_uses - 1) & 1, 256u);
     } else {
         // -------------------------------------------------------------- softmax groups / epilogue ---
         const uint32_t s = warp >> 2, quad = warp & 3, r_in = quad * 32 + lane, gtid = tid & 127;
         const uint32_t lane_base = (quad * 32u) << 16;
         const uint32_t s_tm = tmem + lane_base + s * 128, o_base = tmem + lane_base + 256;
-        uint32_t s_phase = 0, o_uses[2] = {0, 0}, loads = 0;  // loads: tiles the ring has seen before this item
+        uint32_t s_phase = 0, pv = 0, o_phase = 0, loads = 0;  // pv: this stream's P V so far; loads: tiles the ring has seen
         for (uint32_t i = item0; i < item1; ++i) {
             ChunkItem it = load_item(p, i);
             const uint32_t n = it.tile_end - it.tile_begin, x_item = it.tile_begin * kTile;
@@ -431,20 +448,22 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             float m_ref = kNegInf, l = 0.f;
             for (uint32_t j = 0; j < mine; ++j) {
                 const uint32_t t = paired_rows ? j : 2 * j + s;
-                const int32_t x0 = (int32_t)(x_item + t * kTile);
-                wait(bar(kSFull + s), s_phase, 512u);
-                s_phase ^= 1;
-                tc_fence_after();
-                if (busy) {
-                    const bool whole = __all_sync(0xffffffffu, !valid || (vis.b <= x0 && vis.c >= x0 + (int32_t)kTile) || vis.a >= x0 + (int32_t)kTile);
-                    uint32_t r[kTile];
-                    auto fetch = [&]() {
+#pragma unroll 1
+                for (uint32_t h = 0; h < 2; ++h, ++pv) {
+                    constexpr uint32_t N = kTile / 2;
+                    const int32_t x0 = (int32_t)(x_item + t * kTile + h * N);
+                    const uint32_t sp_tm = s_tm + h * N;
+                    wait(bar(kSFull + s * 2 + h), s_phase, 512u);
+                    tc_fence_after();
+                    if (busy) {
+                        const bool whole = __all_sync(0xffffffffu, !valid || (vis.b <= x0 && vis.c >= x0 + (int32_t)N) || vis.a >= x0 + (int32_t)N);
+                        uint32_t r[N];
 #pragma unroll
-                        for (uint32_t c = 0; c < kTile / 32; ++c) tmem_ld32(s_tm + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
+                        for (uint32_t c = 0; c < N / 32; ++c) tmem_ld32(sp_tm + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
                         tc_wait_ld();
                         if (!whole) {
 #pragma unroll
-                            for (uint32_t c = 0; c < kTile / 32; ++c) {
+                            for (uint32_t c = 0; c < N / 32; ++c) {
                                 const int32_t xc = x0 + (int32_t)c * 32;
                                 const uint32_t see = valid ? low_bits(vis.a - xc) | (low_bits(vis.c - xc) & ~low_bits(vis.b - xc)) : 0xFFFFFFFFu;
                                 if (__all_sync(0xffffffffu, see == 0xFFFFFFFFu)) continue;
@@ -453,71 +472,74 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                                     if (!((see >> q) & 1u)) r[c * 32 + q] = 0xFF800000u;  // -inf: weight exactly 0
                             }
                         }
-                    };
-                    fetch();
-                    float mx0 = -3.0e38f, mx1 = -3.0e38f, mx2 = -3.0e38f, mx3 = -3.0e38f;
+                        float mx0 = -3.0e38f, mx1 = -3.0e38f, mx2 = -3.0e38f, mx3 = -3.0e38f;
 #pragma unroll
-                    for (uint32_t q = 0; q < kTile; q += 8) {
-                        mx0 = max3(mx0, __uint_as_float(r[q]), __uint_as_float(r[q + 1]));
-                        mx1 = max3(mx1, __uint_as_float(r[q + 2]), __uint_as_float(r[q + 3]));
-                        mx2 = max3(mx2, __uint_as_float(r[q + 4]), __uint_as_float(r[q + 5]));
-                        mx3 = max3(mx3, __uint_as_float(r[q + 6]), __uint_as_float(r[q + 7]));
-                    }
-                    const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
-                    const float m_new = mx > -3.0e38f ? mx * p.scale_log2 : kNegInf;
-                    const bool grow = valid && m_new > m_ref + kRescaleThreshold;
-                    const float m_old = m_ref;
-                    if (grow) m_ref = m_new;
-                    if (j > 0 && __any_sync(0xffffffffu, grow)) {
-                        const float alpha = fast_exp2(m_old - m_ref);
-                        l *= alpha;
+                        for (uint32_t q = 0; q < N; q += 8) {
+                            mx0 = max3(mx0, __uint_as_float(r[q]), __uint_as_float(r[q + 1]));
+                            mx1 = max3(mx1, __uint_as_float(r[q + 2]), __uint_as_float(r[q + 3]));
+                            mx2 = max3(mx2, __uint_as_float(r[q + 4]), __uint_as_float(r[q + 5]));
+                            mx3 = max3(mx3, __uint_as_float(r[q + 6]), __uint_as_float(r[q + 7]));
+                        }
+                        const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
+                        const float m_new = mx > -3.0e38f ? mx * p.scale_log2 : kNegInf;
+                        const bool grow = valid && m_new > m_ref + kRescaleThreshold;
+                        const float m_old = m_ref;
+                        if (grow) m_ref = m_new;
+                        if ((j > 0 || h > 0) && __any_sync(0xffffffffu, grow)) {
+                            // O has to hold every earlier P V before it is scaled.  The one before the last has completed
+                            // (its half's scores were issued behind it), so the parity is unambiguous.
+                            wait(bar(kODone + s), (pv - 1) & 1, 4096u);
+                            tc_fence_after();
+                            const float alpha = fast_exp2(m_old - m_ref);
+                            l *= alpha;
 #pragma unroll 1
-                        for (uint32_t c = 0; c < D / 32; ++c) {
-                            uint32_t ob[32];
-                            tmem_ld32(o_base + s * 128 + c * 32, ob);
-                            tc_wait_ld();
+                            for (uint32_t c = 0; c < D / 32; ++c) {
+                                uint32_t ob[32];
+                                tmem_ld32(o_base + s * 128 + c * 32, ob);
+                                tc_wait_ld();
 #pragma unroll
-                            for (uint32_t q = 0; q < 32; ++q) ob[q] = __float_as_uint(__uint_as_float(ob[q]) * alpha);
-                            tmem_st32(o_base + s * 128 + c * 32, ob);
+                                for (uint32_t q = 0; q < 32; ++q) ob[q] = __float_as_uint(__uint_as_float(ob[q]) * alpha);
+                                tmem_st32(o_base + s * 128 + c * 32, ob);
+                            }
+                            tc_wait_st();
                         }
-                        tc_wait_st();
-                        fetch();  // rather than keeping the scores in registers across this rare block
-                    }
-                    const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(-m_ref, -m_ref);
-                    float2 acc_a = make_float2(0.f, 0.f), acc_b = make_float2(0.f, 0.f);
+                        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(-m_ref, -m_ref);
+                        float2 acc_a = make_float2(0.f, 0.f), acc_b = make_float2(0.f, 0.f);
 #pragma unroll
-                    for (uint32_t c = 0; c < kTile / 32; ++c) {
-                        uint32_t pk[16];
+                        for (uint32_t c = 0; c < N / 32; ++c) {
+                            uint32_t pk[16];
 #pragma unroll
-                        for (uint32_t q = 0; q < 16; ++q) {
-                            const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c * 32 + 2 * q]), __uint_as_float(r[c * 32 + 2 * q + 1])), sc2, nm2);
-                            float2 w;
-                            w.x = fast_exp2(x.x);
-                            w.y = fast_exp2(x.y);
-                            if (q & 1) acc_b = __fadd2_rn(acc_b, w);
-                            else acc_a = __fadd2_rn(acc_a, w);
-                            pk[q] = pack_f16x2(w.x, w.y);
+                            for (uint32_t q = 0; q < 16; ++q) {
+                                const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c * 32 + 2 * q]), __uint_as_float(r[c * 32 + 2 * q + 1])), sc2, nm2);
+                                float2 w;
+                                w.x = fast_exp2(x.x);
+                                w.y = fast_exp2(x.y);
+                                if (q & 1) acc_b = __fadd2_rn(acc_b, w);
+                                else acc_a = __fadd2_rn(acc_a, w);
+                                pk[q] = pack_f16x2(w.x, w.y);
+                            }
+                            tmem_st16(sp_tm + c * 16, pk);
                         }
-                        tmem_st16(s_tm + c * 16, pk);
+                        const float2 acc = __fadd2_rn(acc_a, acc_b);
+                        l += acc.x + acc.y;
                     }
-                    const float2 acc = __fadd2_rn(acc_a, acc_b);
-                    l += acc.x + acc.y;
+                    // Dead rows of this half, relative to it: [any_a, any_b) and [any_c, end).
+                    const int32_t end = (int32_t)N, gap0 = max(any_a - x0, 0), gap1 = min(any_b - x0, end);
+                    const int32_t tail = any_c - x0;
+                    if (gap0 < gap1 || tail < end) {
+                        const uint32_t load = loads + (paired_rows ? 2 * j + 1 : 4 * j + ((2 * j + 1 < n) ? 2 + s : 1));
+                        const uint32_t slot = load % kSlots;
+                        wait(bar(kFull + slot), (load / kSlots) & 1, 1024u);
+                        uint8_t *v_rows = smem + 2 * kBytes + slot * kBytes + h * (kBytes / 2);
+                        clear_rows<D>(v_rows, gap0, gap1, gtid);
+                        clear_rows<D>(v_rows, max(tail, 0), end, gtid);
+                    }
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(kPFull + s * 2 + h));
                 }
-                // Dead rows of this tile, relative to it: [any_a, any_b) and [any_c, end).
-                const int32_t end = (int32_t)kTile, gap0 = max(any_a - x0, 0), gap1 = min(any_b - x0, end);
-                const int32_t tail = any_c - x0;
-                if (gap0 < gap1 || tail < end) {
-                    uint32_t load = loads + (paired_rows ? 2 * j + 1 : 4 * j + ((2 * j + 1 < n) ? 2 + s : 1));
-                    const uint32_t slot = load % kSlots;
-                    wait(bar(kFull + slot), (load / kSlots) & 1, 1024u);
-                    uint8_t *v_tile = smem + 2 * kBytes + slot * kBytes;
-                    clear_rows<D>(v_tile, gap0, gap1, gtid);
-                    clear_rows<D>(v_tile, max(tail, 0), end, gtid);
-                }
-                tc_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(kPFull + s));
+                s_phase ^= 1;
             }
             loads += 2 * n;
             it = load_item(p, i);  // rather than kept in registers across the tiles
@@ -525,11 +547,10 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             // ---- the item's rows ------------------------------------------------------------------------
             // paired rows: group s has all D dims of its own rows; paired keys: dims [s * D/2, (s + 1) * D/2) of the
             // same rows, from both streams' states.
-            const bool act0 = n > 0 && (paired_rows ? s == 0 : true), act1 = n > 0 && (paired_rows ? s == 1 : n > 1);
             float f0 = 1.f, f1 = 0.f;  // factors of O_own / (O_0, O_1)
             if (!paired_rows) {
                 ml_s[s * kTile + r_in] = make_float2(m_ref, l);
-                if (mine) wait(bar(kOFull + s), o_uses[s] & 1, 2048u);
+                if (mine) wait(bar(kOFull + s), o_phase, 2048u);
                 named_bar_sync(9, 256);
                 const float2 x0 = ml_s[r_in], x1 = ml_s[kTile + r_in];
                 named_bar_sync(10, 256);  // the next item may publish
@@ -538,8 +559,9 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                 f1 = fast_exp2(x1.x - m_ref);
                 l = x0.y * f0 + x1.y * f1;
             } else if (n) {
-                wait(bar(kOFull + s), o_uses[s] & 1, 2048u);
+                wait(bar(kOFull + s), o_phase, 2048u);
             }
+            if (mine) o_phase ^= 1;
             tc_fence_after();
             const bool cut = it.n_parts > 1;
             const float norm = cut ? 1.f : (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));  // a sum that is not a number shows
@@ -624,8 +646,6 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                     if (n > 1) mbar_arrive(bar(kOFree + 1));
                 }
             }
-            if (act0 || (paired_rows && n)) ++o_uses[0];
-            if (act1 || (paired_rows && n)) ++o_uses[1];
             uint32_t again = __ballot_sync(0xffffffffu, valid && !(odd == 0.f) && fabsf(l) <= 3.0e38f && fabsf(m_ref) <= 3.0e38f);
             while (again) {
                 const uint32_t src = __ffs(again) - 1;
