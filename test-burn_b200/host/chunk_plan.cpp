@@ -9,9 +9,12 @@
 namespace mf {
 namespace {
 
-// What an item costs its CTA beyond its tiles (loading q, draining the products, writing the rows), in tiles.
-constexpr uint32_t kItemCost = 2;
-// Shortest piece a unit is cut into when every CTA has several units.
+// Costs in a common unit of about a quarter of a microsecond: a tile of a unit with more than 128 rows (two query tiles on
+// every key tile: 2.1 us, the softmax's pace), a tile of a unit with at most that (1.4 us, the memory's pace), and what
+// an item costs its CTA beyond its tiles (q, draining the products, writing the rows, joining: about 4 us).  With equal
+// costs for all tiles the CTAs that had a mixed step's prompt rows ended 90 us behind the others.
+constexpr uint32_t kRowsTileCost = 8, kKeysTileCost = 5, kItemCost = 16;
+// Shortest piece a unit is cut into when every CTA has several units, in tiles.
 constexpr uint32_t kMinPiece = 2;
 
 }  // namespace
@@ -27,6 +30,7 @@ void build_chunk_plan(const uint32_t *q_lens, const uint32_t *kv_lens, uint32_t 
                       std::vector<uint32_t> &cta_begin)
 {
     const uint32_t per_unit = 2 * (kChunkTile / group), P = page_size;
+    auto tile_cost = [&](const ChunkItem &u) { return u.n_tok > per_unit / 2 ? kRowsTileCost : kKeysTileCost; };
     std::vector<ChunkItem> units;
     uint64_t cost = 0;
     uint32_t tok = 0;
@@ -52,7 +56,7 @@ void build_chunk_plan(const uint32_t *q_lens, const uint32_t *kv_lens, uint32_t 
                     u.n_pages = u.n_sink_pages + (uint32_t)(last / P) - u.first_page + 1;
                     u.tile_end = (uint32_t)(((uint64_t)u.n_pages * P + kChunkTile - 1) / kChunkTile);
                 }
-                cost += u.tile_end + kItemCost;
+                cost += (uint64_t)u.tile_end * tile_cost(u) + kItemCost;
                 units.push_back(u);
             }
         tok += q_lens[b];
@@ -73,27 +77,30 @@ void build_chunk_plan(const uint32_t *q_lens, const uint32_t *kv_lens, uint32_t 
         slots += parts;
         ++counters;
     };
-    // A span boundary usually cuts a unit, and the second piece pays for being an item again.
-    cost += (uint64_t)n_ctas * kItemCost;
+    auto parts_of = [&](const ChunkItem &u, uint32_t most) {
+        const uint32_t tiles = most / tile_cost(u);
+        return std::max(1u, (u.tile_end + tiles - 1) / tiles);
+    };
     uint32_t lo = 1;
     bool pieces = units.size() <= n_ctas;
     if (pieces) {
-        // Few units: one item per CTA, every unit cut into even pieces of at most `lo` tiles, the smallest number
-        // for which there are CTAs enough - unless unequal units leave some CTA more than an equal span would.
-        uint32_t hi = 1;
-        for (const ChunkItem &u : units) hi = std::max(hi, u.tile_end);
+        // Few units: one item per CTA, every unit cut into even pieces that cost at most `lo`, the smallest number for
+        // which there are CTAs enough - unless unequal units leave some CTA more than an equal span would.
+        lo = kRowsTileCost;
+        uint32_t hi = lo;
+        for (const ChunkItem &u : units) hi = std::max(hi, u.tile_end * tile_cost(u));
         while (lo < hi) {
             const uint32_t mid = lo + (hi - lo) / 2;
             uint64_t need = 0;
-            for (const ChunkItem &u : units) need += std::max(1u, (u.tile_end + mid - 1) / mid);
+            for (const ChunkItem &u : units) need += parts_of(u, mid);
             if (need <= n_ctas) hi = mid;
             else lo = mid + 1;
         }
-        pieces = lo + kItemCost <= cost / n_ctas + 2;
+        pieces = lo + kItemCost <= cost / n_ctas + 2 * kItemCost;  // (spans pay an item more per CTA)
     }
     if (pieces) {
         for (const ChunkItem &u : units) {
-            const uint32_t parts = std::max(1u, (u.tile_end + lo - 1) / lo);
+            const uint32_t parts = parts_of(u, lo);
             const size_t first = items.size();
             for (uint32_t i = 0; i < parts; ++i) {
                 ChunkItem it = u;
@@ -106,36 +113,54 @@ void build_chunk_plan(const uint32_t *q_lens, const uint32_t *kv_lens, uint32_t 
         for (uint32_t c = 0; c <= n_ctas; ++c) cta_begin[c] = (uint32_t)std::min<size_t>(c, items.size());
         return;
     }
-    // Spans of equal cost over the list of units, cut where a span ends.
-    uint32_t cta = 0;
-    uint64_t before = 0;  // cost of everything placed so far
-    for (const ChunkItem &u : units) {
-        const size_t first = items.size();
-        uint32_t at = 0;
-        do {
-            // this CTA's span ends at cost * (cta + 1) / n_ctas
-            while (cta + 1 < n_ctas && before >= cost * (cta + 1) / n_ctas) cta_begin[++cta] = (uint32_t)items.size();
-            const uint64_t end = cost * (cta + 1) / n_ctas;
-            const uint64_t room = end > before + kItemCost ? end - before - kItemCost : 0;
-            uint32_t take = u.tile_end - at;
-            if (cta + 1 < n_ctas && take > room) {
-                take = (uint32_t)room;
-                if (take < kMinPiece || u.tile_end - at - take < kMinPiece) take = (uint64_t)take * 2 >= u.tile_end - at ? u.tile_end - at : 0;
-            }
-            if (take == 0 && u.tile_end > at) {  // too little room: the unit goes on in the next CTA
-                before = end;
-                continue;
-            }
-            ChunkItem it = u;
-            it.tile_begin = at;
-            it.tile_end = at + take;
-            items.push_back(it);
-            before += take + kItemCost;
-            at += take;
-        } while (at < u.tile_end);
-        number_parts(first);
+    // Spans over the list of units, cut where a span is full; the smallest span for which the CTAs suffice.  fill() walks the
+    // list with spans of cost `span` and returns how many there are (n_ctas + 1: too many).
+    auto fill = [&](uint64_t span, bool emit) {
+        uint32_t cta = 0;
+        uint64_t room = span;
+        for (const ChunkItem &u : units) {
+            const uint32_t w = tile_cost(u);
+            const size_t first = items.size();
+            uint32_t at = 0;
+            do {
+                const uint32_t rest = u.tile_end - at;
+                uint32_t take = room > kItemCost ? (uint32_t)std::min<uint64_t>(rest, (room - kItemCost) / w) : 0;
+                if (take < rest && rest - take < kMinPiece) take = rest > kMinPiece ? rest - kMinPiece : 0;
+                if (take < rest && take < kMinPiece) take = 0;
+                const bool fits = room >= kItemCost && (take > 0 || rest == 0);
+                if (!fits) {
+                    if (++cta == n_ctas) return n_ctas + 1;
+                    if (emit) cta_begin[cta] = (uint32_t)items.size();
+                    room = span;
+                    continue;
+                }
+                if (emit) {
+                    ChunkItem it = u;
+                    it.tile_begin = at;
+                    it.tile_end = at + take;
+                    items.push_back(it);
+                }
+                room -= kItemCost + (uint64_t)take * w;
+                at += take;
+                if (rest == 0) break;
+            } while (at < u.tile_end);
+            if (emit) number_parts(first);
+        }
+        if (emit)
+            while (cta < n_ctas) cta_begin[++cta] = (uint32_t)items.size();
+        return cta + 1;
+    };
+    uint64_t low = std::max<uint64_t>(cost / n_ctas, kItemCost + kMinPiece * kRowsTileCost), high = low;
+    while (fill(high, false) > n_ctas) {
+        low = high + 1;
+        high += high / 8 + 1;
     }
-    while (cta < n_ctas) cta_begin[++cta] = (uint32_t)items.size();
+    while (low + low / 256 < high) {  // within half a percent
+        const uint64_t mid = low + (high - low) / 2;
+        if (fill(mid, false) > n_ctas) low = mid + 1;
+        else high = mid;
+    }
+    fill(high, true);
 }
 
 }  // namespace mf
