@@ -106,9 +106,9 @@ def test_work_is_spread(mfk):
                                    ([1] * 64, rng.integers(512, 16384, 64), 16, 2, 4096), ([4096], [8192], 16, 2, 0),
                                    ([512, 384] + [1] * 46, rng.integers(600, 8192, 48), 32, 8, 0)):
         items, begin = mfk.build_chunk_plan_host(q, kv, n_heads=hq, n_kv_heads=hkv, page_size=16, n_ctas=148, window=window)
-        # the planner's units: 8 for a tile of a unit with more than 128 rows, 5 for another, 16 for an item
+        # the planner's units: 9 for a tile of a unit with more than 128 rows, 5 for another, 16 for an item
         rows = items[:, 3].astype(int) > TILE // (hq // hkv)
-        cost = (items[:, 9] - items[:, 8]).astype(int) * np.where(rows, 8, 5) + 16
+        cost = (items[:, 9] - items[:, 8]).astype(int) * np.where(rows, 9, 5) + 16
         load = np.array([cost[a:b].sum() for a, b in zip(begin, begin[1:])])
         assert load.max() <= 1.15 * load.mean() + 16, (load.max(), load.mean())
 
