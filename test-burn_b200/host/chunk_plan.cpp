@@ -86,7 +86,7 @@ void build_chunk_plan(const uint32_t *q_lens, const uint32_t *kv_lens, uint32_t 
     if (pieces) {
         // Few units: one item per CTA, every unit cut into even pieces that cost at most `lo`, the smallest number for
         // which there are CTAs enough - unless unequal units leave some CTA more than an equal span would.
-        lo = kRowsTileCost;
+        lo = 2 * kKeysTileCost;  // (the two streams of a small unit take two tiles in about the time of one)
         uint32_t hi = lo;
         for (const ChunkItem &u : units) hi = std::max(hi, u.tile_end * tile_cost(u));
         while (lo < hi) {
