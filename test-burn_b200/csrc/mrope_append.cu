@@ -56,7 +56,7 @@ __device__ __forceinline__ uint2 bytes_of(const Chunk &x, float scale)
 }
 
 constexpr uint32_t kThreads = 256;
-__host__ __device__ constexpr uint32_t in_flight(bool k8) { return k8 ? 2 : 4; }  // chunk pairs a thread has in flight
+__host__ __device__ constexpr uint32_t in_flight(bool k8) { return k8 ? 2 : 3; }  // chunk pairs a thread has in flight
 constexpr uint32_t kVHeads = 8;     // 8-bit V: kv heads transposed at a time
 
 // First block index of sequence b.  The tokens [q_begin[b], q_begin[b + 1]) touch at most (their number) / R + 2 aligned
@@ -65,7 +65,7 @@ __host__ __device__ __forceinline__ uint64_t first_block(uint64_t begin, uint32_
 
 // blockIdx: (block of rows, part of the head slots); the last part of the 8-bit form has the V rows.
 template <uint32_t D, bool K8>
-__global__ void __launch_bounds__(kThreads, 4) mrope_append_kernel(const __grid_constant__ MropeParams p)
+__global__ void __launch_bounds__(kThreads, 5) mrope_append_kernel(const __grid_constant__ MropeParams p)
 {
     constexpr uint32_t R = K8 ? 16 : 8, half = D / 2, cpr = D / 16;  // cpr: chunk pairs per head row
     __shared__ __align__(16) __half cos_s[R * half], sin_s[R * half];
@@ -283,10 +283,12 @@ mf_status launch_mrope(MfContext *ctx, MropeParams &p, const char *what)
     const uint32_t R = K8 ? 16 : 8, cpr = p.head_dim / 16;
     const uint64_t blocks = first_block(p.tokens, p.batch, R) + 1;
     const uint64_t slots = (p.q_rot ? p.n_heads : 0) + (uint64_t)(K8 ? 1 : 2) * p.n_kv_heads;
-    // Prompts: so many parts that a whole block leaves every thread one round of loads.  Decode steps (a token or few per
-    // sequence) have little for a CTA as it is.
+    // Prompts: so many parts that a whole block leaves every thread two rounds of loads (one round: 41 and 18 us for 8.2k
+    // tokens of 32/8 heads and 6.1k tokens into the 8-bit cache, two: 39.6 and 17, no parts at all: 57 and 26).  Decode
+    // steps (a token or few per sequence) have little for a CTA as it is.
+    const uint64_t per_part = 2ull * in_flight(K8) * kThreads;
     uint64_t parts = 1;
-    if (p.tokens >= 4ull * p.batch) parts = std::min<uint64_t>((R * slots * cpr + in_flight(K8) * kThreads - 1) / (in_flight(K8) * kThreads), 64);
+    if (p.tokens >= 4ull * p.batch) parts = std::min<uint64_t>((R * slots * cpr + per_part - 1) / per_part, 64);
     p.slots_per_part = (uint32_t)((slots + parts - 1) / parts);
     parts = (slots + p.slots_per_part - 1) / p.slots_per_part + (K8 ? 1 : 0);
     if (blocks > 0x7FFFFFFFull) return fail(ctx, MF_ERR_INVALID_SHAPE, "%s: %u tokens of %u sequences", what, p.tokens, p.batch);
