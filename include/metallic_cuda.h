@@ -659,7 +659,9 @@ MF_API mf_status mf_paged_gather(MfContext *ctx, const MfPagedKv *cache, uint32_
  * allocates at creation only.  Updates are enqueued on the context's stream; launches that use one
  * plan must not overlap on the GPU (its partial results and tickets are shared by them), whether
  * eager or replayed.  A launch captured into a CUDA graph follows the updates made before its
- * replay; an update itself is refused while the stream is being captured. */
+ * replay (q and out then have to hold max_tokens); an update itself is refused while the stream is
+ * being captured.  A plan takes 39 MB on the device at head_dim 128 (the partial results of units that
+ * several CTAs share), half of that at 64, and 64 bytes per work item. */
 typedef struct MfChunkPlan MfChunkPlan;
 MF_API mf_status mf_chunk_plan_create(MfContext *ctx, const uint32_t *q_lens_host, const uint32_t *kv_lens_host,
                                       uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
@@ -678,7 +680,7 @@ MF_API uint32_t mf_chunk_plan_build_host(const uint32_t *q_lens_host, const uint
                                          uint32_t n_sinks, uint32_t n_ctas, uint32_t *items_out, uint32_t item_capacity,
                                          uint32_t *cta_begin_out);
 /* q and out: f16, 16-byte aligned; element (token t, head h, dim d) at t * stride_t + h * stride_h + d,
- * strides in elements, multiples of 8.  q is rotated already.  scale >= 0. */
+ * strides in elements, multiples of 8; out does not overlap q.  q is rotated already.  scale >= 0. */
 typedef struct MfPagedChunkArgs {
     const void *q;
     void *out;
@@ -687,8 +689,10 @@ typedef struct MfPagedChunkArgs {
 } MfPagedChunkArgs;
 /* Attention of the plan's step over the pages of its sequences (cache->kv_lens is not read: the plan has
  * the lengths).  Page-table entries of pages that no row sees are not read: they may have been given
- * back (mf_page_pool_release_hidden).  head_dim 64 or 128, pages of 8 to 128 rows (a power of two),
- * up to 64 query heads per kv head. */
+ * back (mf_page_pool_release_hidden).  Rows of q and out behind the plan's tokens are not touched.  A key or
+ * value that is not finite shows in the rows that see it and in no other.  The result of a call does not
+ * depend on what else runs (no atomics on values).  head_dim 64 or 128, pages of 8 to 128 rows (a power of
+ * two), up to 64 query heads per kv head. */
 MF_API mf_status mf_paged_chunk_attention(MfContext *ctx, const MfChunkPlan *plan, const MfPagedKv *cache,
                                           const MfPagedChunkArgs *args);
 
@@ -697,7 +701,10 @@ MF_API mf_status mf_paged_chunk_attention(MfContext *ctx, const MfChunkPlan *pla
  * cache row kv_lens[b] - (q_begin[b + 1] - t); its rotation is another matter: frequency j of a head
  * (dims j and j + D/2 in MF_ROPE_MODE_NEOX, 2j and 2j + 1 in MF_ROPE_MODE_NORMAL) turns by row
  * positions[axis[j]][t] of the cos / sin tables.  With equal positions on all axes this is the
- * rotation of mf_paged_kv_append, bit for bit. */
+ * rotation of mf_paged_kv_append, bit for bit.  head_dim 64 or 128, pages of a multiple of 8 rows.
+ * q_begin, kv_lens, positions and the page table are read on the device: a token without a row (its sequence
+ * shorter than its new tokens, a position outside the page table, a page id outside the pool) is not stored,
+ * a position outside the cos / sin tables does not turn its pair, and mf_synchronize reports either. */
 #define MF_MAX_ROPE_AXES 4
 typedef struct MfMropeAppendArgs {
     const void *q, *k, *v;      /* device f16 [tokens, heads * head_dim], rows q/k/v_stride elements apart */

@@ -32,7 +32,6 @@
 //
 // TMEM columns (512): halves 0, 1 of S_0/P_0 [0,64) [64,128), of S_1/P_1 [128,192) [192,256), O_0 [256,384)  O_1 [384,512).
 #include <algorithm>
-#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <new>
@@ -52,7 +51,8 @@ struct MfChunkPlan {
     std::vector<mf::ChunkItem> h_items;
     std::vector<uint32_t> h_begin;
     // [begin_words], [item_capacity] items; two pinned copies used in turn, each guarded by the event
-    // recorded after its upload
+    // recorded after its upload.  One allocation on the device, one on the host.
+    void *device_block = nullptr;
     uint32_t *d_list = nullptr;
     uint32_t *pinned[2] = {nullptr, nullptr};
     cudaEvent_t staged[2] = {nullptr, nullptr};
@@ -69,7 +69,7 @@ constexpr uint32_t kMaxLen = 1u << 30;  // positions and tile arithmetic stay in
 constexpr uint32_t kTile = kChunkTile;
 constexpr uint32_t kThreads = 384;
 constexpr uint32_t kProducerWarp = 8, kIssuerWarp = 9, kQWarp = 11;
-constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr uint64_t kWaitNs = 2000000000ull;  // bits of the status word: the `code` of the wait that ran out (kStatusBadPage is none of them)
 constexpr float kNegInf = -1e30f;
 constexpr float kRescaleThreshold = 8.0f;  // log2 of the largest weight kept in P
 constexpr uint32_t kHalfTile = kTile * 128;
@@ -488,7 +488,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                         if ((j > 0 || h > 0) && __any_sync(0xffffffffu, grow)) {
                             // O has to hold every earlier P V before it is scaled.  The one before the last has completed
                             // (its half's scores were issued behind it), so the parity is unambiguous.
-                            wait(bar(kODone + s), (pv - 1) & 1, 4096u);
+                            wait(bar(kODone + s), (pv - 1) & 1, 16384u);
                             tc_fence_after();
                             const float alpha = fast_exp2(m_old - m_ref);
                             l *= alpha;
@@ -727,6 +727,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     }
 }
 
+auto *chunk_kernel(uint32_t head_dim) { return head_dim == 128 ? chunk_tc_kernel<128> : chunk_tc_kernel<64>; }
+
 mf_status check_lens(MfContext *ctx, const uint32_t *q_lens, const uint32_t *kv_lens, uint32_t batch, uint64_t *tokens,
                      uint32_t *max_kv)
 {
@@ -755,14 +757,10 @@ void mf_chunk_plan_destroy(MfContext *ctx, MfChunkPlan *pl)
     if (!pl) return;
     DeviceScope scope(pl->device);
     if (ctx) cudaStreamSynchronize(ctx->stream);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 2; ++i)
         if (pl->staged[i]) cudaEventDestroy(pl->staged[i]);
-        if (pl->pinned[i]) cudaFreeHost(pl->pinned[i]);
-    }
-    if (pl->d_list) cudaFree(pl->d_list);
-    if (pl->d_acc) cudaFree(pl->d_acc);
-    if (pl->d_ml) cudaFree(pl->d_ml);
-    if (pl->d_tickets) cudaFree(pl->d_tickets);
+    if (pl->pinned[0]) cudaFreeHost(pl->pinned[0]);
+    if (pl->device_block) cudaFree(pl->device_block);
     delete pl;
 }
 
@@ -799,6 +797,8 @@ mf_status mf_chunk_plan_update(MfContext *ctx, MfChunkPlan *pl, const uint32_t *
     st = check_cuda(ctx, cudaMemcpyAsync(pl->d_list, w, 4 * (size_t)pl->begin_words + item_bytes, cudaMemcpyHostToDevice, ctx->stream),
                     "chunk plan: upload");
     if (st != MF_OK) return st;
+    // (every launch leaves the tickets at zero, one whose waits ran out may not)
+    if ((st = check_cuda(ctx, cudaMemsetAsync(pl->d_tickets, 0, 4 * (size_t)pl->n_ctas, ctx->stream), "chunk plan: tickets")) != MF_OK) return st;
     if ((st = check_cuda(ctx, cudaEventRecord(pl->staged[s], ctx->stream), "chunk plan: upload")) != MF_OK) return st;
     pl->next_stage = s ^ 1;
     pl->tokens = (uint32_t)tokens;
@@ -846,17 +846,21 @@ mf_status mf_chunk_plan_create(MfContext *ctx, const uint32_t *q_lens, const uin
     pl->n_ctas = (uint32_t)ctx->sm_count;
     pl->begin_words = (pl->n_ctas + 2 + 15) / 16 * 16;
     pl->item_capacity = chunk_item_capacity(batch, pl->max_tokens, n_kv_heads, n_heads / n_kv_heads, pl->n_ctas);
-    const size_t bytes = 4 * (size_t)pl->begin_words + pl->item_capacity * sizeof(ChunkItem);
-    for (int i = 0; i < 2; ++i) {
-        ok(cudaMallocHost(reinterpret_cast<void **>(&pl->pinned[i]), bytes));
-        ok(cudaEventCreateWithFlags(&pl->staged[i], cudaEventDisableTiming));
+    const size_t list_bytes = (4 * (size_t)pl->begin_words + pl->item_capacity * sizeof(ChunkItem) + 255) / 256 * 256;
+    const size_t rows = (size_t)chunk_slots(pl->n_ctas) * 2 * kTile, acc_bytes = rows * head_dim * 4, ml_bytes = rows * 8;
+    ok(cudaMallocHost(reinterpret_cast<void **>(&pl->pinned[0]), 2 * list_bytes));
+    for (int i = 0; i < 2; ++i) ok(cudaEventCreateWithFlags(&pl->staged[i], cudaEventDisableTiming));
+    ok(cudaMalloc(&pl->device_block, acc_bytes + ml_bytes + list_bytes + 4 * (size_t)pl->n_ctas));
+    if (e == cudaSuccess) {
+        char *at = static_cast<char *>(pl->device_block);
+        pl->pinned[1] = pl->pinned[0] + list_bytes / 4;
+        pl->d_acc = reinterpret_cast<float *>(at);
+        pl->d_ml = reinterpret_cast<float *>(at + acc_bytes);
+        pl->d_list = reinterpret_cast<uint32_t *>(at + acc_bytes + ml_bytes);
+        pl->d_tickets = reinterpret_cast<uint32_t *>(at + acc_bytes + ml_bytes + list_bytes);
     }
-    const size_t rows = (size_t)chunk_slots(pl->n_ctas) * 2 * kTile;
-    ok(cudaMalloc(reinterpret_cast<void **>(&pl->d_list), bytes));
-    ok(cudaMalloc(reinterpret_cast<void **>(&pl->d_acc), rows * head_dim * 4));
-    ok(cudaMalloc(reinterpret_cast<void **>(&pl->d_ml), rows * 8));
-    ok(cudaMalloc(reinterpret_cast<void **>(&pl->d_tickets), 4 * (size_t)pl->n_ctas));
-    if (e == cudaSuccess) ok(cudaMemsetAsync(pl->d_tickets, 0, 4 * (size_t)pl->n_ctas, ctx->stream));
+    // (here rather than at the first launch, which may be inside a stream capture)
+    ok(cudaFuncSetAttribute(chunk_kernel(head_dim), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(head_dim)));
     st = e == cudaSuccess ? mf_chunk_plan_update(ctx, pl, q_lens, kv_lens) : check_cuda(ctx, e, "chunk plan allocation");
     if (st != MF_OK) {
         mf_chunk_plan_destroy(ctx, pl);
@@ -935,15 +939,8 @@ mf_status mf_paged_chunk_attention(MfContext *ctx, const MfChunkPlan *pl, const 
         if (st != MF_OK) return st;
         if (ok && ok1) p.q_tokens = pl->tokens;
     }
-    auto *kern = c->head_dim == 128 ? chunk_tc_kernel<128> : chunk_tc_kernel<64>;
+    auto *kern = chunk_kernel(c->head_dim);
     const uint32_t smem = smem_bytes(c->head_dim);
-    static std::atomic<bool> configured[64][2];
-    const int di = c->head_dim == 128;
-    if (ctx->device >= 64 || !configured[ctx->device][di].load(std::memory_order_acquire)) {
-        st = check_cuda(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "cudaFuncSetAttribute(chunk_tc)");
-        if (st != MF_OK) return st;
-        if (ctx->device < 64) configured[ctx->device][di].store(true, std::memory_order_release);
-    }
     kern<<<pl->n_ctas, kThreads, smem, ctx->stream>>>(tm_k, tm_v, tm_q, tm_q1, p);
     return check_launch(ctx, "chunk_tc_kernel");
 }

@@ -87,16 +87,17 @@ mf_status launch_moves(MfContext *ctx, const PoolRef *pools, uint32_t n_pools, c
 mf_status move_pages(MfContext *ctx, const std::vector<PoolRef> &pools, uint32_t n_pages, const uint32_t *src, const uint32_t *dst,
                      uint32_t n, const char *what)
 {
-    // Destinations are distinct and no source is one: the copies may then run in any order.
-    std::vector<uint8_t> seen(n_pages, 0);
-    for (uint32_t i = 0; i < n; ++i) {
+    for (uint32_t i = 0; i < n; ++i)
         if (src[i] >= n_pages || dst[i] >= n_pages)
             return fail(ctx, MF_ERR_INVALID_OPERATION, "%s: pair %u (%u -> %u) outside the pool of %u pages", what, i, src[i], dst[i], n_pages);
-        if (seen[dst[i]]) return fail(ctx, MF_ERR_INVALID_OPERATION, "%s: page %u is written twice", what, dst[i]);
-        seen[dst[i]] = 1;
-    }
+    // Destinations are distinct and no source is one: the copies may then run in any order.
+    std::vector<uint32_t> written(dst, dst + n);
+    std::sort(written.begin(), written.end());
+    const auto twice = std::adjacent_find(written.begin(), written.end());
+    if (twice != written.end()) return fail(ctx, MF_ERR_INVALID_OPERATION, "%s: page %u is written twice", what, *twice);
     for (uint32_t i = 0; i < n; ++i)
-        if (seen[src[i]]) return fail(ctx, MF_ERR_INVALID_OPERATION, "%s: page %u is read and written", what, src[i]);
+        if (std::binary_search(written.begin(), written.end(), src[i]))
+            return fail(ctx, MF_ERR_INVALID_OPERATION, "%s: page %u is read and written", what, src[i]);
     DeviceScope scope(ctx->device);
     for (size_t p0 = 0; p0 < pools.size(); p0 += kMovePools) {
         const uint32_t np = (uint32_t)std::min<size_t>(kMovePools, pools.size() - p0);

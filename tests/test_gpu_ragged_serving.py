@@ -117,3 +117,74 @@ def test_serving_loop(mfk, foundry):
     assert pool.free_count == POOL
     plans["w"].close()
     pool.close()
+
+
+def test_agrees_with_the_batched_decode(mfk):
+    """One new token per sequence: mf_paged_decode (append and rotation inside, launches overlapping) and the append with
+    equal positions on all axes + chunk attention leave the same rows in the pools and the same attention, up to the two
+    kernels' roundings of the weights (each within 2^-11 + 2^-12 of the weighted mean of |v|, see chunkcases.py)."""
+    f = mfk.Foundry(0, torch.cuda.Stream().cuda_stream)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    kv = [1, 40, 700, 800]
+    pages = torch.randperm(200, generator=g, device="cuda").int()
+    table = pages.view(4, 50).contiguous()
+    lens = torch.tensor(kv, dtype=torch.int32, device="cuda")
+    base = [torch.randn((200, HKV, P, D), generator=g, device="cuda").half() for _ in range(2)]
+    q, k, v = (torch.randn((4, h * D), generator=g, device="cuda").half() for h in (HQ, HKV, HKV))
+    cos, sin = (torch.from_numpy(x.view(np.float16).copy()).cuda() for x in mfk.rope_tables(1e4, D, 1024))
+    a, b = [x.clone() for x in base], [x.clone() for x in base]
+    kw = dict(n_kv_heads=HKV, page_size=P, head_dim=D)
+    plan = f.decode_plan(kv, n_heads=HQ, **kw)
+    chunk = f.chunk_plan([1] * 4, kv, n_heads=HQ, **kw)
+    out_a, out_b, rot = (torch.empty((4, HQ * D), dtype=torch.float16, device="cuda") for _ in range(3))
+    begin = torch.arange(5, dtype=torch.int32, device="cuda")
+    pos = (lens - 1).repeat(3, 1).contiguous()
+    torch.cuda.synchronize()
+    f.set_option(mfk.OPTION_OVERLAP_LAUNCHES, 1)
+    for _ in range(3):  # again and again on the same pools: the same rows are written
+        f.paged_decode(plan, mfk.paged_kv(*a, table, lens, **kw), q, out_a, n_heads=HQ, k=k, v=v, cos=cos, sin=sin, rope=True, append=True)
+        f.paged_mrope_append(mfk.paged_kv(*b, table, lens, **kw), q, k, v, rot, cos, sin, pos, begin, mfk.mrope_axes([16, 24, 24]), n_heads=HQ)
+        f.paged_chunk_attention(chunk, mfk.paged_kv(*b, table, lens, **kw), rot, out_b)
+    f.synchronize()
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+    mean = 4.0  # |v| of normal rows: its weighted mean stays below
+    assert float((out_a.double() - out_b.double()).abs().max()) <= 2 * (2.0 ** -11 + 2.0 ** -12) * mean + 2.0 ** -10 * 4.0
+    plan.close()
+    chunk.close()
+    f.close()
+
+
+def test_pools_beyond_four_gigabytes(mfk, foundry):
+    """Pages whose byte offsets pass 32 bits: append, attention and moves at the far end of 5 GB pools."""
+    n_pages, page = 20500, 128
+    pools = [torch.empty((n_pages, 8, page, D), dtype=torch.float16, device="cuda") for _ in range(2)]
+    far = list(range(n_pages - 9, n_pages))
+    table = torch.tensor([[far[3], far[0], far[5]]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([300], dtype=torch.int32, device="cuda")
+    cache = mfk.paged_kv(*pools, table, lens, n_kv_heads=8, page_size=page, head_dim=D)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    q, k, v = (torch.randn((300, h * D), generator=g, device="cuda").half() for h in (16, 8, 8))
+    cos, sin = torch.ones((1, D // 2), dtype=torch.float16, device="cuda"), torch.zeros((1, D // 2), dtype=torch.float16, device="cuda")
+    begin = torch.tensor([0, 300], dtype=torch.int32, device="cuda")
+    foundry.paged_mrope_append(cache, None, k, v, None, cos, sin, torch.zeros((1, 300), dtype=torch.int32, device="cuda"), begin, bytes(64), n_heads=16)
+    for pool, rows in zip(pools, (k, v)):
+        for t0, pg in ((0, far[3]), (128, far[0]), (256, far[5])):
+            n = min(128, 300 - t0)
+            foundry.synchronize()
+            assert torch.equal(pool[pg, :, :n], rows.view(300, 8, D)[t0:t0 + n].transpose(0, 1))
+    src, dst = np.array([far[3], far[0], far[5]], np.uint32), np.array([far[8], 1, far[7]], np.uint32)
+    foundry.paged_move_pages(mfk.kv_layers([cache]), src, dst)
+    table.copy_(torch.from_numpy(dst.astype(np.int32))[None])
+    torch.cuda.synchronize()
+    plan = foundry.chunk_plan([300], [300], n_heads=16, n_kv_heads=8, head_dim=D, page_size=page)
+    out = torch.empty_like(q)
+    foundry.paged_chunk_attention(plan, cache, q, out)
+    foundry.synchronize()
+    kk, vv = (x.view(300, 8, D).transpose(0, 1).repeat_interleave(2, 0).double() for x in (k, v))
+    see = torch.ones((300, 300), dtype=torch.bool, device="cuda").tril()
+    w = torch.softmax((q.view(300, 16, D).transpose(0, 1).double() @ kk.transpose(1, 2) * D ** -0.5).masked_fill(~see, -float("inf")), -1)
+    want, mean = (w @ vv).transpose(0, 1), (w @ vv.abs()).transpose(0, 1)
+    got = out.view(300, 16, D).double()
+    assert bool(((got - want).abs() <= 2.0 ** -11 * want.abs() + (2.0 ** -11 + 2.0 ** -12) * mean + 2.0 ** -16).all())
+    plan.close()
