@@ -9,6 +9,10 @@
 // sin rows of its tokens into shared memory once for all heads, and finds its sequence once.  A thread turns two 16-byte
 // chunks at a time (append.cuh), several in flight.  V bytes of the 8-bit cache are transposed through shared memory: a
 // whole block goes out as 16-byte words, a part of one byte by byte.
+//
+// Measured: 8.2k tokens of 32/8 heads of 128 (210 MB) 39.6 us, 5.3 TB/s, 0.81 of the copy rate; 6.1k tokens of 16/2 heads
+// into the 8-bit cache (47 MB) 17 us - two thirds of it launch, the chain of loads before a CTA's first row (sequence,
+// page, positions, tables) and the drain; one token of each of 64 sequences 3.5 us.
 #include <cuda_fp8.h>
 
 #include <algorithm>
