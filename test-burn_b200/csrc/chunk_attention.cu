@@ -75,7 +75,7 @@ namespace mf {
 namespace {
 
 constexpr uint32_t kMaxGroup = 64;
-constexpr uint32_t kMaxLen = 1u << 30;  // positions and tile arithmetic stay inside 32 bits
+constexpr uint32_t kMaxLen = kChunkMaxLen;
 constexpr uint32_t kTile = kChunkTile;
 constexpr uint32_t kThreads = 384;
 constexpr uint32_t kProducerWarp = 8, kIssuerWarp = 9, kQWarp = 11;
@@ -910,7 +910,7 @@ mf_status mf_paged_chunk_attention(MfContext *ctx, const MfChunkPlan *pl, const 
         return fail(ctx, MF_ERR_INVALID_SHAPE, "paged chunk attention: q, out and the pools must be 16-byte aligned");
     if ((a->q_stride_t | a->q_stride_h | a->out_stride_t | a->out_stride_h) & 7u)
         return fail(ctx, MF_ERR_INVALID_SHAPE, "paged chunk attention: strides must be multiples of 8 elements");
-    if (!(a->scale >= 0.f) || !std::isfinite(a->scale))
+    if (!(a->scale >= 0.f) || !std::isfinite(a->scale * 1.4426950408889634f))
         return fail(ctx, MF_ERR_INVALID_OPERATION, "paged chunk attention: scale %g", (double)a->scale);
     if (pl->max_tokens == 0 || !a->q || !a->out) return MF_OK;
     DeviceScope scope(ctx->device);

@@ -7,6 +7,7 @@
 namespace mf {
 
 constexpr uint32_t kChunkTile = 128;  // keys per tile and query rows per stream
+constexpr uint32_t kChunkMaxLen = 1u << 30;  // positions and tile arithmetic stay inside 32 bits
 
 // A unit is the attention of up to 2 * (128 / G) consecutive new tokens of one sequence with the G query heads of one
 // kv head: the rows (token, head) fill one or two 128-row query tiles ("streams").  The keys some row of the unit sees

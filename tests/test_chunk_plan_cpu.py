@@ -121,3 +121,9 @@ def test_arguments_without_a_meaning(mfk):
     for bad in ((1, 7, 2, 16, 1), (1, 8, 0, 16, 1), (1, 8, 2, 0, 1), (1, 8, 2, 16, 0), (1, 0, 2, 16, 1), (1, 130, 2, 16, 1)):
         batch, hq, hkv, page, ctas = bad
         assert f(p, p, batch, hq, hkv, page, 0, 0, ctas, None, 0, begin.ctypes.data) == 0
+
+
+@pytest.mark.parametrize("q_len,kv_len", [((1 << 30) + 1, 1 << 30), (0xFFFFFFFF, 5), (1, (1 << 30) + 1), (1, 0xFFFFFFFF)])
+def test_lengths_past_the_limit(mfk, q_len, kv_len):
+    items, begin = mfk.build_chunk_plan_host([q_len], [kv_len], n_heads=8, n_kv_heads=2, page_size=16, n_ctas=4)
+    assert len(items) == 0 and not begin.any()
