@@ -556,8 +556,8 @@ class Foundry:
         """Causal (windowed) attention of the plan's new tokens; q and out: f16 [tokens, Hq*D] or [tokens, Hq, D], any
         token and head strides that are multiples of 8."""
         d = cache.head_dim
-        qt, qh = _head_strides(q, plan, d, "q")
-        ot, oh = _head_strides(out, plan, d, "out")
+        qt, qh = _head_strides(q, plan, d, "q", self.device)
+        ot, oh = _head_strides(out, plan, d, "out", self.device)
         a = _CHUNK_ARGS.pack(q.data_ptr(), out.data_ptr(), qt, qh, ot, oh, d ** -0.5 if scale is None else scale)
         self.check(lib.mf_paged_chunk_attention(self._h, plan._h, C.byref(cache), a))
 
@@ -568,21 +568,28 @@ class Foundry:
         int32 [n_axes, tokens], q_begin: int32 [batch + 1], axes: the axis of every frequency (see mrope_axes)."""
         d, tokens, n_kv = cache.head_dim, k.shape[0], cache.n_kv_heads
         half = d // 2
-        k_stride, v_stride = _row_stride(k, tokens, n_kv * d, "k"), _row_stride(v, tokens, n_kv * d, "v")
-        q_stride = _row_stride(q, tokens, n_heads * d, "q") if q is not None else 0
-        rot_stride = _row_stride(q_rot, tokens, n_heads * d, "q_rot") if q_rot is not None else 0
+        dev = self.device
+        q_ptr = q_stride = rot_ptr = rot_stride = 0
+        k_stride, v_stride = _row_stride(k, tokens, n_kv * d, "k", dev), _row_stride(v, tokens, n_kv * d, "v", dev)
+        if q is not None:
+            q_ptr, q_stride = q.data_ptr(), _row_stride(q, tokens, n_heads * d, "q", dev)
+        if q_rot is not None:
+            rot_ptr, rot_stride = q_rot.data_ptr(), _row_stride(q_rot, tokens, n_heads * d, "q_rot", dev)
         rows = cos.shape[0]
-        if not (cos.numel() == rows * half == sin.numel() and cos.is_contiguous() and sin.is_contiguous()):
-            raise MetalError(2, f"mrope append: cos / sin must be [rows, {half}]")
-        p_strides = positions.stride()
-        if len(p_strides) != 2 or positions.shape[1] != tokens or p_strides[1] != 1 or positions.element_size() != 4:
-            raise MetalError(2, f"mrope append: positions must be int32 [n_axes, {tokens}]")
-        if q_begin.shape != (cache.batch + 1,) or q_begin.element_size() != 4 or q_begin.stride() != (1,):
-            raise MetalError(2, f"mrope append: q_begin must be int32 [{cache.batch + 1}]")
+        if not (cos.numel() == rows * half == sin.numel() and cos.is_contiguous() and sin.is_contiguous() and
+                _kinds[cos.dtype] == _F16 == _kinds[sin.dtype] and cos.get_device() == dev == sin.get_device()):
+            raise MetalError(2, f"mrope append: cos / sin must be f16 [rows, {half}] on device {dev}")
+        p_shape, p_strides = positions.shape, positions.stride()
+        if len(p_shape) != 2 or p_shape[1] != tokens or p_strides[1] != 1 or _kinds[positions.dtype] != _INT32 or \
+                positions.get_device() != dev:
+            raise MetalError(2, f"mrope append: positions must be int32 [n_axes, {tokens}] on device {dev}")
+        if q_begin.shape != (cache.batch + 1,) or q_begin.stride() != (1,) or _kinds[q_begin.dtype] != _INT32 or \
+                q_begin.get_device() != dev:
+            raise MetalError(2, f"mrope append: q_begin must be int32 [{cache.batch + 1}] on device {dev}")
         if len(axes) != half:
             raise MetalError(2, f"mrope append: {len(axes)} axes for {half} frequencies")
-        n_axes = positions.shape[0]
-        a = _MROPE_ARGS.pack(_ptr(q) or 0, k.data_ptr(), v.data_ptr(), _ptr(q_rot) or 0, cos.data_ptr(), sin.data_ptr(),
+        n_axes = p_shape[0]
+        a = _MROPE_ARGS.pack(q_ptr, k.data_ptr(), v.data_ptr(), rot_ptr, cos.data_ptr(), sin.data_ptr(),
                              positions.data_ptr(), q_begin.data_ptr(), q_stride, k_stride, v_stride, rot_stride, tokens, n_heads,
                              n_axes, p_strides[0] if n_axes > 1 else tokens, rows, rope_mode, bytes(axes))
         fn = lib.mf_paged_kv8_mrope_append if isinstance(cache, MfPagedKv8) else lib.mf_paged_mrope_append
@@ -909,25 +916,42 @@ class ChunkPlan:
             pass
 
 
-def _head_strides(x, plan: ChunkPlan, d: int, name: str):
+# A tensor of another type would be read as if it were of the right one, one of the host's memory would fault.
+_F16, _INT32 = 1, 2
+
+
+class _Kinds(dict):
+    """torch dtype -> _F16, _INT32 or 0 (by name: PyTorch is not imported for it)."""
+
+    def __missing__(self, dtype):
+        self[dtype] = kind = {"torch.float16": _F16, "torch.int32": _INT32, "torch.uint32": _INT32}.get(str(dtype), 0)
+        return kind
+
+
+_kinds = _Kinds()
+
+
+def _head_strides(x, plan: ChunkPlan, d: int, name: str, device: int):
     """(token, head) strides of f16 [tokens, heads * d] or [tokens, heads, d]."""
     shape, st = x.shape, x.stride()
-    if shape[0] >= plan.tokens and st[-1] == 1 and x.element_size() == 2:
+    if len(shape) > 1 and shape[0] >= plan.tokens and st[-1] == 1 and _kinds[x.dtype] == _F16 and x.get_device() == device:
         if len(shape) == 2 and shape[1] == plan.n_heads * d:
             return st[0], d
         if len(shape) == 3 and shape[1] == plan.n_heads and shape[2] == d:
             return st[0], st[1]
-    raise MetalError(2, f"paged chunk attention: {name} {tuple(shape)} for {plan.tokens} tokens of {plan.n_heads} heads of {d}")
+    raise MetalError(2, f"paged chunk attention: {name} {tuple(shape)} {x.dtype} on {x.device} for f16 {plan.tokens} tokens of "
+                        f"{plan.n_heads} heads of {d} on device {device}")
 
 
-def _row_stride(x, rows: int, cols: int, name: str) -> int:
+def _row_stride(x, rows: int, cols: int, name: str, device: int) -> int:
     """Row stride of f16 [rows, cols] with unit column stride."""
-    if x.numel() == rows * cols and x.is_contiguous() and x.element_size() == 2 and x.dim() == 2:
-        return cols
-    st = x.stride()
-    if x.shape != (rows, cols) or st[-1] != 1 or x.element_size() != 2:
-        raise MetalError(2, f"mrope append: {name} must be f16 [{rows}, {cols}] with unit column stride")
-    return st[0]
+    if _kinds[x.dtype] == _F16 and x.get_device() == device:
+        st = x.stride()
+        if st == (cols, 1) and x.numel() == rows * cols:
+            return cols
+        if x.shape == (rows, cols) and st[1] == 1:
+            return st[0] if rows > 1 else cols
+    raise MetalError(2, f"mrope append: {name} must be f16 [{rows}, {cols}] with unit column stride on device {device}")
 
 
 def mrope_axes(sections, interleaved: bool = False) -> bytes:

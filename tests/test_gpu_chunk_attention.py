@@ -258,6 +258,7 @@ def test_refusals(mfk, foundry):
     call("InvalidOperation", scale=-1.0)
     call("InvalidOperation", scale=float("nan"))
     call("InvalidOperation", scale=float("inf"))
+    call("InvalidOperation", scale=3e38)  # finite, but not in the exponent of two
     call("InvalidOperation", cache=other(page_table_stride=6))
     call("InvalidShape", cache=other(batch=3))
     call("InvalidShape", cache=other(page_size=32))
@@ -282,3 +283,15 @@ def test_another_current_device_is_put_back(mfk, foundry):
     assert torch.cuda.current_device() == 0
     foundry.synchronize()
     check(out, case)
+
+
+def test_other_types_and_memories_are_refused(mfk, foundry):
+    case = ChunkCase(hq=8, hkv=2, d=128, page=16, q_lens=[2, 1], kv_lens=[100, 50])
+    plan, cache, out = case.plan(foundry), case.cache(mfk), torch.zeros_like(case.q)
+    for q, o in ((case.q.bfloat16(), out), (case.q, out.bfloat16()), (case.q.cpu(), out), (case.q, out.cpu()),
+                 (case.q.view(torch.int16), out), (case.q.flatten(), out)):
+        with pytest.raises(mfk.MetalError) as e:
+            foundry.paged_chunk_attention(plan, cache, q, o)
+        assert e.value.kind == "InvalidShape"
+    foundry.synchronize()
+    assert not bool(out.any())

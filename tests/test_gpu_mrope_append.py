@@ -230,3 +230,20 @@ def test_refusals(mfk, foundry):
     foundry.paged_mrope_append(mfk.paged_kv(dev[0], dev[1], table, lens, n_kv_heads=2, page_size=16, head_dim=128), *empty.values(), n_heads=8)
     foundry.synchronize()
     assert torch.equal(before, dev[0])
+
+
+def test_other_types_and_memories_are_refused(mfk, foundry):
+    case = Case(mfk, hq=8, hkv=2, d=128, page=16, q_lens=[4], kv_lens=[40])
+    dev = [p.cuda() for p in case.pools]
+    before = dev[0].clone()
+    table, lens = case.table.cuda(), torch.tensor([40], dtype=torch.int32).cuda()
+    cache = mfk.paged_kv(dev[0], dev[1], table, lens, n_kv_heads=2, page_size=16, head_dim=128)
+    good = dict(q=case.q.cuda(), k=case.k.cuda(), v=case.v.cuda(), q_rot=torch.zeros((4, 1024), dtype=torch.float16, device="cuda"),
+                cos=case.cos.cuda(), sin=case.sin.cuda(), positions=case.pos.cuda(), q_begin=case.begin.cuda())
+    for name, x in good.items():
+        for bad in (x.cpu(), x.bfloat16() if x.dtype == torch.float16 else x.float()):
+            with pytest.raises(mfk.MetalError) as e:
+                foundry.paged_mrope_append(cache, *(good | {name: bad}).values(), case.axes, n_heads=8)
+            assert e.value.kind == "InvalidShape", name
+    foundry.synchronize()
+    assert torch.equal(before, dev[0]) and not bool(good["q_rot"].any())
