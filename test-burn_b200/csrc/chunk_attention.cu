@@ -38,7 +38,9 @@
 //     part of the exponentials as a cubic on the FMA pipe: none is faster over long blocks.
 //   decode (64 sequences, window 4 096, 177 MB): 41 us in a graph, 4.3 TB/s; from the first tile (4 us after the launch) to
 //     the last (33 us) the keys stream at 0.9 of the copy rate, the rest is start, drain and joining of cut units.
-//   one token, 1 028 keys: 10 us, of which the last piece's joining is 2 and fence and ticket 1.
+//   one token, 1 028 keys: 9.3 us, of which the last piece's joining is 2 and fence and ticket 1.  A half tile in which no
+//     row sees a key (behind the last one) is left out: 10.4 without that, five drafted tokens of each of 8 sequences
+//     14.2 instead of 15.5 (a first pass over the softmax costs 1.4).
 //
 // TMEM columns (512): halves 0, 1 of S_0/P_0 [0,64) [64,128), of S_1/P_1 [128,192) [192,256), O_0 [256,384)  O_1 [384,512).
 #include <algorithm>
@@ -386,6 +388,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             if (n == 0) continue;
             const bool paired_rows = it.n_tok > half_tok;
             const uint32_t tiles = paired_rows ? n : (n + 1 - s) / 2;
+            // the item's last tile, if no row sees its second half (the softmax groups leave that half out, too)
+            const uint32_t half_tile = visible(p, it, it.pos0 + (int32_t)it.n_tok - 1).c <= (int32_t)(it.tile_end * kTile - kTile / 2) ? n - 1 : n;
             const uint64_t q_desc = smem_desc(q_smem + (paired_rows ? s * kBytes : 0), 16, 1024);
             // paired rows: K V K V ..., for both streams; paired keys: K0 K1 V0 V1 ..., a last single tile K0 V0
             Place k = paired_rows ? base : ahead(base, s), v = k;
@@ -422,10 +426,12 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                     wait(bar(kPFull + s * 2 + h), p_phase, 64u);
                     if (j == 0 && h == 0 && o_uses) wait(bar(kOFree + s), (o_uses - 1) & 1, 128u);
                     tc_fence_after();
+                    if (h == 0 || (paired_rows ? j : 2 * j + s) != half_tile) {
 #pragma unroll
-                    for (uint32_t kk = 0; kk < kTile / 32; ++kk)
-                        tc_mma_ts_elected(elected, tmem + 256 + s * 128, tmem + s * 128 + h * 64 + kk * 8,
-                                          v_desc + ((kk * 2 * kGroupStride) >> 4), kIdescPV, (j > 0 || h > 0 || kk > 0) ? 1u : 0u);
+                        for (uint32_t kk = 0; kk < kTile / 32; ++kk)
+                            tc_mma_ts_elected(elected, tmem + 256 + s * 128, tmem + s * 128 + h * 64 + kk * 8,
+                                              v_desc + ((kk * 2 * kGroupStride) >> 4), kIdescPV, (j > 0 || h > 0 || kk > 0) ? 1u : 0u);
+                    }
                     tc_commit_elected(elected, bar(kODone + s));
                     if (h == 1) release(v.slot);
                     if (more) scores(h);
@@ -472,7 +478,9 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                     const uint32_t sp_tm = s_tm + h * N;
                     wait(bar(kSFull + s * 2 + h), s_phase, 512u);
                     tc_fence_after();
-                    if (busy) {
+                    // (a tile's first half is not left out: the item's first product also clears O)
+                    const bool seen = h == 0 || any_c > x0;
+                    if (busy && seen) {
                         const bool whole = __all_sync(0xffffffffu, !valid || (vis.b <= x0 && vis.c >= x0 + (int32_t)N) || vis.a >= x0 + (int32_t)N);
                         uint32_t r[N];
 #pragma unroll
@@ -543,7 +551,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                     // Dead rows of this half, relative to it: [any_a, any_b) and [any_c, end).
                     const int32_t end = (int32_t)N, gap0 = max(any_a - x0, 0), gap1 = min(any_b - x0, end);
                     const int32_t tail = any_c - x0;
-                    if (gap0 < gap1 || tail < end) {
+                    if (seen && (gap0 < gap1 || tail < end)) {
                         const uint32_t load = loads + (paired_rows ? 2 * j + 1 : 4 * j + ((2 * j + 1 < n) ? 2 + s : 1));
                         const uint32_t slot = load % kSlots;
                         wait(bar(kFull + slot), (load / kSlots) & 1, 1024u);

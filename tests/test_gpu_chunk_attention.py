@@ -64,6 +64,22 @@ def test_against_definition(mfk, foundry, name):
     plan.close()
 
 
+@pytest.mark.parametrize("page", [8, 64, 128])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 5)])
+@pytest.mark.parametrize("q_len", [1, 20])
+def test_last_half_tiles(mfk, foundry, page, window, sinks, q_len):
+    """Lengths around the halves of a tile (64 keys): a last half that no row sees is left out, whatever it holds."""
+    lens = [x + y for x in (0, 128, 256) for y in (1, 20, 63, 64, 65, 83, 84, 127, 128)]
+    lens = [n for n in lens if n >= q_len]
+    case = ChunkCase(hq=8, hkv=1, d=128 if page == 64 else 64, page=page, q_lens=[q_len] * len(lens), kv_lens=lens, window=window, sinks=sinks)
+    plan, out = case.plan(foundry), torch.empty_like(case.q)
+    for _ in range(2):
+        out.fill_(float("nan"))
+        foundry.paged_chunk_attention(plan, case.cache(mfk), case.q, out)
+        foundry.synchronize()
+        check(out, case)
+
+
 def test_scores_far_apart(mfk, foundry):
     """Scores of several hundred (weights that underflow, maxima that keep moving) and a scale of the caller's."""
     case = ChunkCase(hq=8, hkv=2, d=128, page=16, q_lens=[130, 1], kv_lens=[700, 1500], spread=30.0)
