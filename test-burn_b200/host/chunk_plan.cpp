@@ -122,7 +122,7 @@ void build_chunk_plan(const uint32_t *q_lens, const uint32_t *kv_lens, uint32_t 
             const uint32_t w = tile_cost(u);
             const size_t first = items.size();
             uint32_t at = 0;
-            do {
+            for (bool whole = false; !whole;) {
                 const uint32_t rest = u.tile_end - at;
                 uint32_t take = room > kItemCost ? (uint32_t)std::min<uint64_t>(rest, (room - kItemCost) / w) : 0;
                 if (take < rest && rest - take < kMinPiece) take = rest > kMinPiece ? rest - kMinPiece : 0;
@@ -132,7 +132,7 @@ void build_chunk_plan(const uint32_t *q_lens, const uint32_t *kv_lens, uint32_t 
                     if (++cta == n_ctas) return n_ctas + 1;
                     if (emit) cta_begin[cta] = (uint32_t)items.size();
                     room = span;
-                    continue;
+                    continue;  // (a unit without tiles, too: its rows are written)
                 }
                 if (emit) {
                     ChunkItem it = u;
@@ -142,8 +142,8 @@ void build_chunk_plan(const uint32_t *q_lens, const uint32_t *kv_lens, uint32_t 
                 }
                 room -= kItemCost + (uint64_t)take * w;
                 at += take;
-                if (rest == 0) break;
-            } while (at < u.tile_end);
+                whole = at >= u.tile_end;
+            }
             if (emit) number_parts(first);
         }
         if (emit)

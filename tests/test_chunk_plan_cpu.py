@@ -127,3 +127,19 @@ def test_arguments_without_a_meaning(mfk):
 def test_lengths_past_the_limit(mfk, q_len, kv_len):
     items, begin = mfk.build_chunk_plan_host([q_len], [kv_len], n_heads=8, n_kv_heads=2, page_size=16, n_ctas=4)
     assert len(items) == 0 and not begin.any()
+
+
+@pytest.mark.parametrize("n_ctas", [1, 7, 148])
+def test_units_without_keys_are_in_the_plan(mfk, n_ctas):
+    """New tokens of a sequence without rows come out as zeros: someone has to write them, wherever a span ends."""
+    rng = np.random.default_rng(5)
+    for batch in (1, 60, 300):
+        kv_lens = np.where(rng.random(batch) < 0.5, 0, rng.integers(1, 900, batch))
+        q_lens = rng.integers(0, 40, batch)
+        items, begin = mfk.build_chunk_plan_host(q_lens, kv_lens, n_heads=14, n_kv_heads=2, page_size=16, n_ctas=n_ctas)
+        assert begin[0] == 0 and begin[-1] == len(items) and (np.diff(begin.astype(int)) >= 0).all()
+        first = items[items[:, 8] == 0]  # the piece of a unit that starts at its first tile
+        written = np.zeros((2, q_lens.sum()), int)
+        for it in first:
+            written[it[1], it[2]:it[2] + it[3]] += 1
+        assert (written == 1).all()
