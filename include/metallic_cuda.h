@@ -708,7 +708,7 @@ MF_API mf_status mf_paged_chunk_attention(MfContext *ctx, const MfChunkPlan *pla
 #define MF_MAX_ROPE_AXES 4
 typedef struct MfMropeAppendArgs {
     const void *q, *k, *v;      /* device f16 [tokens, heads * head_dim], rows q/k/v_stride elements apart */
-    void *q_rot;                /* device f16, like q; may be NULL (q is then not read and may be NULL) */
+    void *q_rot;                /* device f16, like q, or q itself; may be NULL (q is then not read and may be NULL) */
     const void *cos, *sin;      /* device f16 [table_rows, head_dim/2] */
     const uint32_t *positions;  /* device [n_axes, position_stride] */
     const uint32_t *q_begin;    /* device [batch + 1], q_begin[0] = 0, q_begin[batch] = tokens */

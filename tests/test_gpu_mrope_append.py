@@ -247,3 +247,56 @@ def test_other_types_and_memories_are_refused(mfk, foundry):
             assert e.value.kind == "InvalidShape", name
     foundry.synchronize()
     assert torch.equal(before, dev[0]) and not bool(good["q_rot"].any())
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_captured_in_place_on_another_stream(mfk, bits):
+    """q may be turned where it is; a captured call reads lengths and positions anew at each replay."""
+    stream = torch.cuda.Stream()
+    f = mfk.Foundry(0, stream.cuda_stream)
+    case = Case(mfk, hq=8, hkv=2, d=128, page=16, q_lens=[20, 3], kv_lens=[40, 30], bits=bits)
+    dev, table = [p.cuda() for p in case.pools], case.table.cuda()
+    lens, pos, q = torch.tensor(case.kv_lens, dtype=torch.int32).cuda(), case.pos.cuda(), case.q.cuda()
+    k, v, cos, sin, begin = case.k.cuda(), case.v.cuda(), case.cos.cuda(), case.sin.cuda(), case.begin.cuda()
+    if bits == 16:
+        cache = mfk.paged_kv(dev[0], dev[1], table, lens, n_kv_heads=2, page_size=16, head_dim=128)
+    else:
+        cache = mfk.paged_kv8(*dev, table, lens, n_kv_heads=2, page_size=16)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        f.paged_mrope_append(cache, q, k, v, q, cos, sin, pos, begin, case.axes, n_heads=8)
+    for kv_lens, shift in (([40, 30], 0), ([33, 17], 5)):
+        case.kv_lens, case.pos = kv_lens, case.pos.add(shift) % case.rows
+        case.pools = [p.cpu().clone() for p in dev]
+        want_q, want = case.expected()
+        lens.copy_(torch.tensor(kv_lens, dtype=torch.int32))
+        pos.copy_(case.pos)
+        q.copy_(case.q)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        f.synchronize()
+        assert np.array_equal(q.cpu().numpy().view(np.uint16), want_q.view(np.uint16))
+        for a, b in zip(dev, want):
+            assert np.array_equal(a.cpu().numpy().view(np.uint8), b.view(np.uint8))
+    del graph
+    f.close()
+
+
+def test_rows_that_are_not_finite_in_the_8_bit_cache(mfk, foundry):
+    """Infinities and NaN are quantised as the one-axis append does it, and stay in their row."""
+    case = Case(mfk, hq=4, hkv=2, d=128, page=16, q_lens=[37], kv_lens=[90], bits=8, mode=1)
+    case.pos[:] = torch.arange(53, 90, dtype=torch.int32)
+    for t, (x, value) in enumerate(((case.k, float("inf")), (case.k, float("nan")), (case.v, -float("inf")), (case.v, float("nan")))):
+        x[5 * t + 1, 7] = value
+    _, dev = case.run(mfk, foundry)
+    want = [p.cuda() for p in case.pools]
+    table, lens = case.table.cuda(), torch.tensor([90], dtype=torch.int32).cuda()
+    args = [x.cuda() for x in (case.q, case.k, case.v)] + [torch.empty((4, 37, 128), dtype=torch.float16, device="cuda"),
+                                                         case.cos.cuda(), case.sin.cuda()]
+    foundry.paged_kv8_append(mfk.paged_kv8(*want, table, lens, n_kv_heads=2, page_size=16), *args, n_heads=4, rope_mode=1, seq=0,
+                             position_offset=53, seq_len=37)
+    foundry.synchronize()
+    for a, b in zip(dev, want):
+        assert np.array_equal(a.view(np.uint8), b.cpu().numpy().view(np.uint8))
