@@ -311,3 +311,14 @@ def test_other_types_and_memories_are_refused(mfk, foundry):
         assert e.value.kind == "InvalidShape"
     foundry.synchronize()
     assert not bool(out.any())
+
+
+def test_sequences_without_keys_among_many(mfk, foundry):
+    """Rows that see nothing come out as zeros wherever their units fall in the CTAs' spans."""
+    kv_lens = [0 if i % 3 == 1 else 40 + 37 * (i % 11) for i in range(60)]
+    q_lens = [i % 4 if kv else 3 for i, kv in enumerate(kv_lens)]
+    case = ChunkCase(hq=56, hkv=8, d=128, page=128, q_lens=q_lens, kv_lens=kv_lens)
+    plan, out = case.plan(foundry), torch.full_like(case.q, float("nan"))
+    foundry.paged_chunk_attention(plan, case.cache(mfk), case.q, out)
+    foundry.synchronize()
+    check(out, case)
