@@ -18,7 +18,7 @@
 //   warps 0-3, 4-7  softmax groups (one thread per row = TMEM lane)   warp 8   TMA producer, one copy per page and tile
 //   warps 9, 10     issue the products of streams 0, 1                warp 11  loads q, allocates TMEM
 //
-// K and V tiles share one ring in the order in which the products want them.  A (page, kv head) run lands as
+// K and V tiles share one ring in the order in which the products want them (chunk_ring.hpp).  A (page, kv head) run lands as
 // [8-row group][half][8 rows][128 bytes], so the 128 rows of a tile are evenly spaced 8-row groups whatever the page
 // size, and both operands (K by rows, V by columns) take one descriptor per tile.
 //
@@ -50,6 +50,7 @@
 #include <vector>
 
 #include "chunk_plan.hpp"
+#include "chunk_ring.hpp"
 #include "internal.hpp"
 #include "ptx.cuh"
 #include "tcgen05.cuh"
@@ -372,16 +373,12 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         const uint32_t s = warp - kIssuerWarp, elected = elect_one_sync();
         constexpr uint32_t kIdescQK = instr_desc_f16(kTile, kTile / 2, 0), kIdescPV = instr_desc_f16(kTile, D, 1);
         constexpr uint32_t kGroupStride = 16 * D;  // bytes between 8-row groups of a K or V tile
-        struct Place {  // of a tile in the ring
-            uint32_t slot, phase;
-        };
-        auto ahead = [&](Place at, uint32_t by) {
-            at.slot += by;
-            if (at.slot >= kSlots) at.slot -= kSlots, at.phase ^= 1;
-            return at;
+        RingReader<kSlots> reader;
+        auto landed = [&](uint32_t slot, uint32_t phase) { wait(bar(kFull + slot), phase, 16u); };
+        auto pass = [&](uint32_t slot) {
+            if (elected) mbar_arrive(bar(kFull + kSlots + slot));
         };
         uint32_t q_phase = 0, p_phase = 0, o_uses = 0;
-        Place base{0, 0};
         for (uint32_t i = item0; i < item1; ++i) {
             const ChunkItem it = load_item(p, i);
             const uint32_t n = it.tile_end - it.tile_begin;
@@ -391,22 +388,19 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             // the item's last tile, if no row sees its second half (the softmax groups leave that half out, too)
             const uint32_t half_tile = visible(p, it, it.pos0 + (int32_t)it.n_tok - 1).c <= (int32_t)(it.tile_end * kTile - kTile / 2) ? n - 1 : n;
             const uint64_t q_desc = smem_desc(q_smem + (paired_rows ? s * kBytes : 0), 16, 1024);
-            // paired rows: K V K V ..., for both streams; paired keys: K0 K1 V0 V1 ..., a last single tile K0 V0
-            Place k = paired_rows ? base : ahead(base, s), v = k;
-            auto release = [&](uint32_t slot) {
-                tc_commit_elected(elected, bar(kFull + kSlots + slot));
-                if (!paired_rows) tc_commit_elected(elected, bar(kFull + kSlots + slot));  // for the other stream too
-            };
+            uint32_t k = 0, v = 0;  // slots of the stream's K and V tile
+            auto next = [&]() { return reader.next(paired_rows, n, s, landed, pass); };
+            auto release = [&](uint32_t slot) { tc_commit_elected(elected, bar(kFull + kSlots + slot)); };
             auto scores = [&](uint32_t h) {
-                wait(bar(kFull + k.slot), k.phase, 16u);
-                const uint64_t k_desc = smem_desc(ring + k.slot * kBytes + h * 8 * kGroupStride, 16, kGroupStride);
+                if (h == 0) k = next();
+                const uint64_t k_desc = smem_desc(ring + k * kBytes + h * 8 * kGroupStride, 16, kGroupStride);
                 tc_fence_after();
 #pragma unroll
                 for (uint32_t kk = 0; kk < D / 16; ++kk)
                     tc_mma_ss_elected(elected, tmem + s * 128 + h * 64, q_desc + (((kk >> 2) * kHalfTile + (kk & 3) * 32) >> 4),
                                       k_desc + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4), kIdescQK, kk > 0);
                 tc_commit_elected(elected, bar(kSFull + s * 2 + h));
-                if (h == 1) release(k.slot);
+                if (h == 1) release(k);
             };
             wait(bar(kQFull), q_phase, 32u);
             q_phase ^= 1;
@@ -417,12 +411,10 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             if (tiles <= 1) tc_commit_elected(elected, bar(kQFree));
             for (uint32_t j = 0; j < tiles; ++j) {
                 const bool more = j + 1 < tiles;
-                v = ahead(k, paired_rows || 2 * j + 1 >= n ? 1 : 2);
-                if (more) k = ahead(k, paired_rows ? 2 : 4);
 #pragma unroll
                 for (uint32_t h = 0; h < 2; ++h) {
-                    if (h == 0) wait(bar(kFull + v.slot), v.phase, 16u);
-                    const uint64_t v_desc = smem_desc(ring + v.slot * kBytes + h * 8 * kGroupStride, 1024, kGroupStride);
+                    if (h == 0) v = next();
+                    const uint64_t v_desc = smem_desc(ring + v * kBytes + h * 8 * kGroupStride, 1024, kGroupStride);
                     wait(bar(kPFull + s * 2 + h), p_phase, 64u);
                     if (j == 0 && h == 0 && o_uses) wait(bar(kOFree + s), (o_uses - 1) & 1, 128u);
                     tc_fence_after();
@@ -433,7 +425,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                                               v_desc + ((kk * 2 * kGroupStride) >> 4), kIdescPV, (j > 0 || h > 0 || kk > 0) ? 1u : 0u);
                     }
                     tc_commit_elected(elected, bar(kODone + s));
-                    if (h == 1) release(v.slot);
+                    if (h == 1) release(v);
                     if (more) scores(h);
                 }
                 p_phase ^= 1;
@@ -441,9 +433,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                 if (j + 2 == tiles) tc_commit_elected(elected, bar(kQFree));
             }
             o_uses += tiles > 0;
-            const uint32_t skip = (2 * n) % kSlots;
-            base.phase ^= ((2 * n) / kSlots) & 1;
-            base = ahead(base, skip);
+            reader.finish(n, landed, pass);
         }
         // The products have to be over before the TMEM goes back (they are, unless a wait ran out).
         if (o_uses) wait(bar(kOFull + s), (o_uses - 1) & 1, 256u);
@@ -552,8 +542,9 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                     const int32_t end = (int32_t)N, gap0 = max(any_a - x0, 0), gap1 = min(any_b - x0, end);
                     const int32_t tail = any_c - x0;
                     if (seen && (gap0 < gap1 || tail < end)) {
-                        const uint32_t load = loads + (paired_rows ? 2 * j + 1 : 4 * j + ((2 * j + 1 < n) ? 2 + s : 1));
-                        const uint32_t slot = load % kSlots;
+                        // (the stream has waited for every load up to this tile's K, at most two in front of its V: the slot's
+                        // use before this one is over, and the parity cannot be mistaken)
+                        const uint32_t load = loads + ring_v_load(paired_rows, n, s, j), slot = load % kSlots;
                         wait(bar(kFull + slot), (load / kSlots) & 1, 1024u);
                         uint8_t *v_rows = smem + 2 * kBytes + slot * kBytes + h * (kBytes / 2);
                         clear_rows<D>(v_rows, gap0, gap1, gtid);
