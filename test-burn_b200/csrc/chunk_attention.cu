@@ -16,7 +16,7 @@
 // the other half and the other stream; a group waits for nothing but its own two halves.
 //
 //   warps 0-3, 4-7  softmax groups (one thread per row = TMEM lane)   warp 8   TMA producer, one copy per page and tile
-//   warps 9, 10     issue the products of streams 0, 1                warp 11  loads q, allocates TMEM
+//   warps 9, 10     issue the products of streams 0, 1                warp 11  loads q, prepares V tiles, allocates TMEM
 //
 // K and V tiles share one ring in the order in which the products want them (chunk_ring.hpp).  A (page, kv head) run lands as
 // [8-row group][half][8 rows][128 bytes], so the 128 rows of a tile are evenly spaced 8-row groups whatever the page
@@ -26,9 +26,11 @@
 // 256 and are rounded to f16 for the product (2^-11 of each), sums, maxima and accumulators are f32.
 //
 // Rows of a tile that no row of the unit sees (the end of the cache, the edge of the window) are cleared in V: their
-// weight is zero, but zero times a stale NaN is not.  A value row that some rows see and others do not can only hurt the
-// others when it is not finite; then the output is not finite either, and such a row is walked again key by key
-// (walk_row).
+// weight is zero, but zero times a stale NaN is not.  For the same reason elements that are not finite are taken out of the
+// value rows that some rows of the unit see and others do not (along the diagonal and the window's edge: at most as many
+// keys as the unit has tokens, each; none for a single token), and added to the rows that do see them when the item's rows
+// are in memory (add_hidden).  What every row sees stays as it is.  Warp 11 does both while the softmax groups are at work
+// (done by the groups it is 53 instead of 44 us for a prompt step of 14/2 heads of 64, window 512).
 //
 // What bounds it (measured on a B200):
 //   long prompts (6.8k new tokens over 8k keys, 16/2 heads of 128; 319 GFLOP): 305 us in a short burst at 1.83 GHz, 354 us
@@ -93,24 +95,28 @@ enum Bar : uint32_t {
     kSFull = 0,   // [stream * 2 + half] scores of the next tile's half are in S
     kPFull = 4,   // [stream * 2 + half] weights are in P, O has been rescaled if needed
     kODone = 8,   // [stream] a P V has completed (one phase per half tile)
-    kOFull = 10,  // [stream] the item's last P V has completed
+    kOFull = 10,  // [stream] the item's last P V has completed (2 arrivals: with the issuing warp's own)
     kOFree = 12,  // [stream] the item's O has been read (8 arrivals)
     kQFull = 14,
     kQFree = 15,  // 2 arrivals: the streams' last Q K^T of the item
-    kFull = 16    // [slots], then empty [slots] (2 arrivals: the streams)
+    kFull = 16    // [slots], then empty [slots] (3 arrivals: the streams and warp 11), then fit [slots] (warp 11 is through with it)
 };
-__host__ __device__ constexpr uint32_t num_bars(uint32_t d) { return kFull + 2 * ring_slots(d); }
+__host__ __device__ constexpr uint32_t num_bars(uint32_t d) { return kFull + 3 * ring_slots(d); }
 constexpr uint32_t kMlBytes = 2 * kTile * 8;  // (m, l) of the two streams' rows
+// Words behind the barriers: TMEM address, abort flag, "last piece of the unit", and the last four items (their number + 1)
+// in which elements were taken out of V rows.  (Warp 11 is at most three items ahead of a softmax group: an item's q goes to
+// shared memory when the one before has been multiplied, and that waits for the weights of the one before it.)
+enum Word : uint32_t { kTmem = 0, kAbort = 1, kLast = 2, kTaken = 4, kNumWords = 8 };
 __host__ __device__ constexpr uint32_t smem_bytes(uint32_t d)
 {
-    return tile_bytes(d) * (2 + ring_slots(d)) + kMlBytes + num_bars(d) * 8 + 16;
+    return tile_bytes(d) * (2 + ring_slots(d)) + kMlBytes + num_bars(d) * 8 + kNumWords * 4;
 }
 static_assert(smem_bytes(128) <= 227 * 1024 && smem_bytes(64) <= 227 * 1024, "shared memory");
 
 struct ChunkParams {
     const __half *q;
     __half *out;
-    const __half *k_pool, *v_pool;  // walk_row only
+    const __half *v_pool;  // add_hidden only
     const uint32_t *page_table;
     const uint32_t *list;  // cta_begin, then the items
     float *acc, *ml;
@@ -166,45 +172,139 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return d;
 }
 
-// sum_x 2^(s_x - m) V[x][d0 .. d0 + dims) over the columns of the item that the row sees, key by key; one warp, result
-// in lanes * dims / 32 consecutive dims.  Rare: only for rows whose product with the whole tile was not finite.
+// Columns of a unit's page list by who sees them.  [gap0, gap1) and what lies behind `end`: no row.  [sink0, sink1),
+// [edge0, edge1), [diag0, diag1): some rows.  All others: every row.  (Rows only gain keys at the diagonal and lose keys at
+// the window's edge: the first and the last row have them all.)
+struct Cuts {
+    int32_t gap0, gap1, end;
+    int32_t sink0, sink1, edge0, edge1, diag0, diag1;
+    // whether the V tile at column x has such rows; its second half is not used when no row sees it
+    __device__ __forceinline__ bool tile(int32_t x) const
+    {
+        const int32_t y = used(x);
+        return end < y || max(gap0, x) < min(gap1, y) || max(sink0, x) < min(sink1, y) || max(edge0, x) < min(edge1, y) ||
+               max(diag0, x) < min(diag1, y);
+    }
+    __device__ __forceinline__ int32_t used(int32_t x) const { return x + (int32_t)(end > x + (int32_t)kTile / 2 ? kTile : kTile / 2); }
+};
+__device__ __forceinline__ Cuts cuts_of(const ChunkParams &p, const ChunkItem &it)
+{
+    const Visible first = visible(p, it, it.pos0), last = visible(p, it, it.pos0 + (int32_t)it.n_tok - 1);
+    const int32_t any_b = visible(p, it, max(it.pos0, 0)).b;
+    Cuts c;
+    c.gap0 = last.a;
+    c.gap1 = any_b;
+    c.end = last.c;
+    c.sink0 = min(last.a, first.c);
+    c.sink1 = last.a;
+    c.edge0 = max(any_b, last.a);
+    c.edge1 = min(last.b, last.c);
+    c.diag0 = max(max(first.c, any_b), last.b);
+    c.diag1 = last.c;
+    return c;
+}
+
+// Makes the V tile at column x fit for the products, by one warp: rows that no row of the unit sees become 0, and so do
+// elements that are not finite in rows that some of them see.  Returns whether there were such elements.
 template <uint32_t D>
-__device__ __noinline__ void walk_row(const ChunkParams &p, uint32_t item, const __half *q, int32_t pos, float m, uint32_t d0,
-                                      uint32_t dims, float (&acc)[D / 32])
+__device__ __noinline__ bool prepare_values(uint8_t *tile, const Cuts cuts, int32_t x)
+{
+    constexpr uint32_t C = D / 8, kStep = 32 / C;  // 16-byte units per row, rows a step
+    const uint32_t lane = threadIdx.x & 31, c = lane % C;
+    const int32_t y = cuts.used(x);
+    auto at = [&](int32_t col) {
+        const uint32_t r = (uint32_t)(col - x);
+        return reinterpret_cast<uint4 *>(tile + (r >> 3) * (16 * D) + (c >> 3) * 1024 + (r & 7) * 128 + (c & 7) * 16);
+    };
+    auto clear = [&](int32_t lo, int32_t hi) {
+        for (int32_t col = max(lo, x) + (int32_t)(lane / C); col < min(hi, y); col += kStep) *at(col) = make_uint4(0, 0, 0, 0);
+    };
+    clear(cuts.gap0, cuts.gap1);
+    clear(cuts.end, y);
+    bool found = false;
+    // an exponent of all ones carries into the sign's place
+    auto odd = [](uint32_t w) { return ((w & 0x7FFF7FFFu) + 0x04000400u) & 0x80008000u; };
+    auto without = [&](uint32_t w) {
+        const uint32_t o = odd(w);
+        return w & ~((o & 0x8000u ? 0xFFFFu : 0u) | (o & 0x80000000u ? 0xFFFF0000u : 0u));
+    };
+    auto take_out = [&](int32_t lo, int32_t hi) {
+        constexpr int32_t kBatch = 8;
+        hi = min(hi, y);
+        for (int32_t col = max(lo, x) + (int32_t)(lane / C); col < hi; col += kBatch * kStep) {
+            uint4 v[kBatch];
+#pragma unroll
+            for (int32_t k = 0; k < kBatch; ++k) {
+                v[k] = make_uint4(0, 0, 0, 0);
+                if (col + k * (int32_t)kStep < hi) v[k] = *at(col + k * (int32_t)kStep);
+            }
+            uint32_t any = 0;
+#pragma unroll
+            for (int32_t k = 0; k < kBatch; ++k) any |= odd(v[k].x) | odd(v[k].y) | odd(v[k].z) | odd(v[k].w);
+            if (any) {
+                found = true;
+#pragma unroll
+                for (int32_t k = 0; k < kBatch; ++k)
+                    if (odd(v[k].x) | odd(v[k].y) | odd(v[k].z) | odd(v[k].w))
+                        *at(col + k * (int32_t)kStep) = make_uint4(without(v[k].x), without(v[k].y), without(v[k].z), without(v[k].w));
+            }
+        }
+    };
+    take_out(cuts.sink0, cuts.sink1);
+    take_out(cuts.edge0, cuts.edge1);
+    take_out(cuts.diag0, cuts.diag1);
+    fence_proxy_async();
+    return __any_sync(0xffffffffu, found);
+}
+
+// What prepare_values took out, added to the rows that see it: a warp's 32 rows, `dims` dims from d0 on.  Such an element
+// decides its row's output in that dim whatever its weight is (the weight of a visible key is positive): added as it is.
+// to: element 0 of the lane's row (f16), or of its partial result (f32, in groups of four dims); null: no row.
+template <uint32_t D, bool CUT>
+__device__ __noinline__ void add_hidden(const ChunkParams &p, uint32_t item, int32_t pos, uint32_t d0, uint32_t dims, void *to)
 {
     const ChunkItem it = load_item(p, item);
-    const uint32_t lane = threadIdx.x & 31, E = dims / 32, P = 1u << p.page_shift;
     const Visible vis = visible(p, it, pos);
-#pragma unroll
-    for (uint32_t e = 0; e < D / 32; ++e) acc[e] = 0.f;
-    const int32_t x0 = it.tile_begin * kTile, x1 = it.tile_end * kTile;
-    for (uint32_t part = 0; part < 2; ++part) {
-        const int32_t lo = max(x0, part ? vis.b : 0), hi = min(x1, part ? vis.c : vis.a);
+    const Cuts cuts = cuts_of(p, it);
+    const uint32_t lane = threadIdx.x & 31, E = dims / 32, P = 1u << p.page_shift;
+    __syncwarp();  // the rows were written by other lanes of the warp
+    for (uint32_t k = 0; k < 3; ++k) {
+        const int32_t lo = max((int32_t)(it.tile_begin * kTile), k == 0 ? cuts.sink0 : k == 1 ? cuts.edge0 : cuts.diag0);
+        const int32_t hi = min((int32_t)(it.tile_end * kTile), k == 0 ? cuts.sink1 : k == 1 ? cuts.edge1 : cuts.diag1);
         for (int32_t x = lo; x < hi; ++x) {
             const uint32_t entry = page_entry(it, (uint32_t)x >> p.page_shift);
             const uint32_t page = entry < p.pt_stride ? p.page_table[(size_t)it.seq * p.pt_stride + entry] : 0xFFFFFFFFu;
             if (page >= p.n_pages) continue;
-            const size_t row = ((((size_t)page * p.n_kv_heads + it.kvh) << p.page_shift) + ((uint32_t)x & (P - 1))) * D;
-            float s = 0.f;
-            for (uint32_t d = lane; d < D; d += 32) s = fmaf(__half2float(q[d]), __half2float(p.k_pool[row + d]), s);
+            const __half *v = p.v_pool + ((((size_t)page * p.n_kv_heads + it.kvh) << p.page_shift) + ((uint32_t)x & (P - 1))) * D + d0;
+            float value[D / 32];
+            bool odd = false;
 #pragma unroll
-            for (uint32_t o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            const float w = fast_exp2(fmaf(s, p.scale_log2, -m));
-            for (uint32_t e = 0; e < E; ++e) acc[e] = fmaf(w, __half2float(p.v_pool[row + d0 + lane * E + e]), acc[e]);
+            for (uint32_t e = 0; e < D / 32; ++e) {
+                value[e] = e < E ? __half2float(v[e * 32 + lane]) : 0.f;
+                odd |= !(fabsf(value[e]) <= 65504.f);
+            }
+            if (!__any_sync(0xffffffffu, odd)) continue;
+            uint32_t rows = __ballot_sync(0xffffffffu, to && (x < vis.a || (x >= vis.b && x < vis.c)));
+            while (rows) {
+                const uint32_t src = __ffs(rows) - 1;
+                rows &= rows - 1;
+                void *row = reinterpret_cast<void *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), src));
+#pragma unroll
+                for (uint32_t e = 0; e < D / 32; ++e) {
+                    const uint32_t d = e * 32 + lane;
+                    if (fabsf(value[e]) <= 65504.f) continue;
+                    if (CUT) {
+                        float *o = static_cast<float *>(row) + (size_t)(d / 4) * (2 * kTile) * 4 + d % 4;
+                        __stcg(o, __ldcg(o) + value[e]);
+                    } else {
+                        __half *o = static_cast<__half *>(row) + d;
+                        *o = __float2half_rn(__half2float(*o) + value[e]);
+                    }
+                }
+            }
         }
     }
-}
-
-// Rows [dead0, dead1) of a V tile are cleared by one softmax group (128 threads).
-template <uint32_t D>
-__device__ __noinline__ void clear_rows(uint8_t *v_tile, int32_t dead0, int32_t dead1, uint32_t gtid)
-{
-    constexpr uint32_t C = D / 8;  // 16-byte units per row
-    for (uint32_t i = gtid; i < (uint32_t)max(dead1 - dead0, 0) * C; i += 128) {
-        const uint32_t r = dead0 + i / C, c = i % C;
-        *reinterpret_cast<uint4 *>(v_tile + (r >> 3) * (16 * D) + (c >> 3) * 1024 + (r & 7) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-    }
-    fence_proxy_async();
+    __syncwarp();
 }
 
 template <uint32_t D>
@@ -218,7 +318,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     float2 *ml_s = reinterpret_cast<float2 *>(smem + kBytes * (2 + kSlots));  // [stream][row]
     const uint32_t bars = q_smem + kBytes * (2 + kSlots) + kMlBytes;
     volatile uint32_t *words = reinterpret_cast<volatile uint32_t *>(smem + kBytes * (2 + kSlots) + kMlBytes + num_bars(D) * 8);
-    volatile uint32_t *abort_flag = words + 1;
+    volatile uint32_t *abort_flag = words + kAbort;
     auto bar = [&](uint32_t i) { return bars + i * 8; };
     // (the warp's number by a shuffle: known to be the same in all its lanes, so that what the issuing warp computes stays
     // in uniform registers)
@@ -237,16 +337,18 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         }
         for (uint32_t s = 0; s < 2; ++s) {
             mbar_init(bar(kODone + s), 1);
-            mbar_init(bar(kOFull + s), 1);
+            mbar_init(bar(kOFull + s), 2);
             mbar_init(bar(kOFree + s), 8);
         }
         mbar_init(bar(kQFull), 1);
         mbar_init(bar(kQFree), 2);
         for (uint32_t s = 0; s < kSlots; ++s) {
             mbar_init(bar(kFull + s), 1);
-            mbar_init(bar(kFull + kSlots + s), 2);
+            mbar_init(bar(kFull + kSlots + s), 3);
+            mbar_init(bar(kFull + 2 * kSlots + s), 1);
         }
         *abort_flag = 0;
+        for (uint32_t x = kTaken; x < kNumWords; ++x) words[x] = 0;
         mbar_fence_init();
         fence_proxy_async();
     }
@@ -257,7 +359,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *words;
+    const uint32_t tmem = words[kTmem];
 
     auto wait = [&](uint32_t b, uint32_t parity, uint32_t code) {
         if (mbar_try_wait(b, parity)) return;
@@ -325,8 +427,29 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         if (lane == 0 && *abort_flag)
             for (uint32_t s = 0; s < kSlots; ++s) mbar_wait_bounded(bar(kFull + s), s < slot ? phase : phase ^ 1, kWaitNs / 16);
     } else if (warp == kQWarp) {
-        // ------------------------------------------------------------------------- q (whole warp) ---
-        uint32_t used = 0;
+        // ------------------------------------------------------------- q and V tiles (whole warp) ---
+        uint32_t used = 0, slot = 0, phase = 0;
+        // This item's loads in turn, like the streams: a tile that some row must not see in part is made fit for the products.
+        auto prepare = [&](uint32_t i, const ChunkItem &it) {
+            const uint32_t n = it.tile_end - it.tile_begin;
+            const bool paired_rows = it.n_tok > half_tok;
+            const Cuts cuts = cuts_of(p, it);
+            for (uint32_t load = 0; load < 2 * n; ++load) {
+                wait(bar(kFull + slot), phase, 8u);
+                const uint32_t t = ring_v_tile(paired_rows, n, load);
+                const int32_t x = (int32_t)((it.tile_begin + t) * kTile);
+                if (t < n && cuts.tile(x)) {
+                    const bool found = prepare_values<D>(smem + (2 + slot) * kBytes, cuts, x);
+                    __syncwarp();
+                    if (found && lane == 0) words[kTaken + used % 4] = i + 1;
+                }
+                if (lane == 0) {
+                    mbar_arrive(bar(kFull + 2 * kSlots + slot));
+                    mbar_arrive(bar(kFull + kSlots + slot));
+                }
+                if (++slot == kSlots) slot = 0, phase ^= 1;
+            }
+        };
         // A replayed launch can meet a plan with more tokens than q had when it was captured: then without the maps.
         const bool by_map = __ldg(p.list + p.begin_words - 1) <= p.q_tokens;
         for (uint32_t i = item0; i < item1; ++i) {
@@ -348,6 +471,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                                             (int32_t)h, bar(kQFull));
                 }
                 __syncwarp();
+                prepare(i, it);
                 continue;
             }
             constexpr uint32_t C = D / 8;
@@ -364,6 +488,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(kQFull));
+            prepare(i, it);
         }
     } else if (warp >= kIssuerWarp) {
         // -------------------------------------------------------- the products of one stream (whole warp) ---
@@ -386,7 +511,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             const bool paired_rows = it.n_tok > half_tok;
             const uint32_t tiles = paired_rows ? n : (n + 1 - s) / 2;
             // the item's last tile, if no row sees its second half (the softmax groups leave that half out, too)
-            const uint32_t half_tile = visible(p, it, it.pos0 + (int32_t)it.n_tok - 1).c <= (int32_t)(it.tile_end * kTile - kTile / 2) ? n - 1 : n;
+            const Cuts cuts = cuts_of(p, it);
+            const uint32_t half_tile = cuts.end <= (int32_t)(it.tile_end * kTile - kTile / 2) ? n - 1 : n;
             const uint64_t q_desc = smem_desc(q_smem + (paired_rows ? s * kBytes : 0), 16, 1024);
             uint32_t k = 0, v = 0;  // slots of the stream's K and V tile
             auto next = [&]() { return reader.next(paired_rows, n, s, landed, pass); };
@@ -413,7 +539,12 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                 const bool more = j + 1 < tiles;
 #pragma unroll
                 for (uint32_t h = 0; h < 2; ++h) {
-                    if (h == 0) v = next();
+                    if (h == 0) {
+                        v = next();
+                        // (a slot's use is handed back by warp 11 when that is through with it: its phase cannot be two behind)
+                        if (cuts.tile((int32_t)((it.tile_begin + (paired_rows ? j : 2 * j + s)) * kTile)))
+                            wait(bar(kFull + 2 * kSlots + v), reader.last_phase(), 1024u);
+                    }
                     const uint64_t v_desc = smem_desc(ring + v * kBytes + h * 8 * kGroupStride, 1024, kGroupStride);
                     wait(bar(kPFull + s * 2 + h), p_phase, 64u);
                     if (j == 0 && h == 0 && o_uses) wait(bar(kOFree + s), (o_uses - 1) & 1, 128u);
@@ -429,7 +560,10 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                     if (more) scores(h);
                 }
                 p_phase ^= 1;
-                if (!more) tc_commit_elected(elected, bar(kOFull + s));
+                if (!more) {
+                    tc_commit_elected(elected, bar(kOFull + s));
+                    if (elected) mbar_arrive(bar(kOFull + s));  // (what warp 11 has written is the softmax groups' to read)
+                }
                 if (j + 2 == tiles) tc_commit_elected(elected, bar(kQFree));
             }
             o_uses += tiles > 0;
@@ -443,7 +577,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         const uint32_t lane_base = (quad * 32u) << 16;
         const uint32_t s_tm = tmem + lane_base + s * 128, o_base = tmem + lane_base + 256;
         const uint32_t row_tok = r_in / G, row_g = r_in - row_tok * G;  // row = (token, query head)
-        uint32_t s_phase = 0, pv = 0, o_phase = 0, loads = 0;  // pv: this stream's P V so far; loads: tiles the ring has seen
+        uint32_t s_phase = 0, pv = 0, o_phase = 0;  // pv: this stream's P V so far
         for (uint32_t i = item0; i < item1; ++i) {
             ChunkItem it = load_item(p, i);
             const uint32_t n = it.tile_end - it.tile_begin, x_item = it.tile_begin * kTile;
@@ -454,9 +588,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             const uint32_t tok = tok_first + (valid ? row_tok : 0), head = it.kvh * G + (valid ? row_g : 0);
             const int32_t pos = it.pos0 + (int32_t)tok;
             const Visible vis = visible(p, it, pos);
-            // columns that some row of the unit sees: [0, any_a), [any_b, any_c)
-            const Visible v_last = visible(p, it, it.pos0 + (int32_t)it.n_tok - 1);
-            const int32_t any_a = v_last.a, any_b = visible(p, it, max(it.pos0, 0)).b, any_c = v_last.c;
+            const int32_t any_c = visible(p, it, it.pos0 + (int32_t)it.n_tok - 1).c;  // columns from here on: no row of the unit
             const uint32_t mine = paired_rows ? n : (n + 1 - s) / 2;
             float m_ref = kNegInf, l = 0.f;
             for (uint32_t j = 0; j < mine; ++j) {
@@ -538,18 +670,6 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                         const float2 acc = __fadd2_rn(acc_a, acc_b);
                         l += acc.x + acc.y;
                     }
-                    // Dead rows of this half, relative to it: [any_a, any_b) and [any_c, end).
-                    const int32_t end = (int32_t)N, gap0 = max(any_a - x0, 0), gap1 = min(any_b - x0, end);
-                    const int32_t tail = any_c - x0;
-                    if (seen && (gap0 < gap1 || tail < end)) {
-                        // (the stream has waited for every load up to this tile's K, at most two in front of its V: the slot's
-                        // use before this one is over, and the parity cannot be mistaken)
-                        const uint32_t load = loads + ring_v_load(paired_rows, n, s, j), slot = load % kSlots;
-                        wait(bar(kFull + slot), (load / kSlots) & 1, 1024u);
-                        uint8_t *v_rows = smem + 2 * kBytes + slot * kBytes + h * (kBytes / 2);
-                        clear_rows<D>(v_rows, gap0, gap1, gtid);
-                        clear_rows<D>(v_rows, max(tail, 0), end, gtid);
-                    }
                     tc_wait_st();
                     tc_fence_before();
                     __syncwarp();
@@ -558,7 +678,6 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                 s_phase ^= 1;
             }
             if (i + 1 < item1) prefetch_item(p, i + 1);
-            loads += 2 * n;
             it = load_item(p, i);  // rather than kept in registers across the tiles
 
             // ---- the item's rows ------------------------------------------------------------------------
@@ -587,9 +706,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             const uint32_t d0 = paired_rows ? 0 : s * (D / 2), dims = paired_rows ? D : D / 2;
             const uint32_t slot_row = (paired_rows ? s * kTile : 0) + r_in;
             // partial results lie by row inside a group of four dims, so that neighbouring threads write neighbouring words
-            float4 *part = reinterpret_cast<float4 *>(p.acc) + ((size_t)it.slot * (D / 4) + d0 / 4) * (2 * kTile) + slot_row;
+            float4 *part_row = reinterpret_cast<float4 *>(p.acc) + ((size_t)it.slot * (D / 4) + d0 / 4) * (2 * kTile) + slot_row;
             __half *dst = p.out + (it.tok0 + (uint64_t)tok) * p.out_stride_t + (uint64_t)head * p.out_stride_h + d0;
-            float odd = 0.f;  // NaN: a value that is not finite
             if (busy) {
                 // Rows go out four lanes to a row: the lanes of a quad swap their 16-byte blocks, lane q then has block q
                 // of each of the quad's rows and four lanes store 64 consecutive bytes.
@@ -619,13 +737,11 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                             for (uint32_t q = 0; q < 32; ++q) o[q] = fmaf(__uint_as_float(o1[q]), f1, o[q]);
                         }
                     }
-#pragma unroll
-                    for (uint32_t q = 0; q < 32; ++q) odd = fmaf(o[q], 0.f, odd);
                     if (cut) {
                         if (valid) {
 #pragma unroll
                             for (uint32_t q = 0; q < 32; q += 4)
-                                __stcg(part + (c * 8 + q / 4) * (2 * kTile), make_float4(o[q], o[q + 1], o[q + 2], o[q + 3]));
+                                __stcg(part_row + (c * 8 + q / 4) * (2 * kTile), make_float4(o[q], o[q + 1], o[q + 2], o[q + 3]));
                         }
                         continue;
                     }
@@ -663,24 +779,10 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                     if (n > 1) mbar_arrive(bar(kOFree + 1));
                 }
             }
-            uint32_t again = __ballot_sync(0xffffffffu, valid && !(odd == 0.f) && fabsf(l) <= 3.0e38f && fabsf(m_ref) <= 3.0e38f);
-            while (again) {
-                const uint32_t src = __ffs(again) - 1;
-                again &= again - 1;
-                const uint32_t w_tok = __shfl_sync(0xffffffffu, tok, src), w_head = __shfl_sync(0xffffffffu, head, src);
-                const float w_m = __shfl_sync(0xffffffffu, m_ref, src), w_norm = __shfl_sync(0xffffffffu, norm, src);
-                float acc[D / 32];
-                walk_row<D>(p, i, p.q + (it.tok0 + (uint64_t)w_tok) * p.q_stride_t + (uint64_t)w_head * p.q_stride_h, it.pos0 + (int32_t)w_tok,
-                            w_m, d0, dims, acc);
-                const uint32_t E = dims / 32;
-                for (uint32_t e = 0; e < E; ++e) {
-                    const uint32_t d = lane * E + e;
-                    if (cut)
-                        __stcg(p.acc + (((size_t)it.slot * (D / 4) + (d0 + d) / 4) * (2 * kTile) + (paired_rows ? s * kTile : 0) + quad * 32 + src) * 4 + d % 4, acc[e]);
-                    else
-                        p.out[(it.tok0 + (uint64_t)w_tok) * p.out_stride_t + (uint64_t)w_head * p.out_stride_h + d0 + d] = __float2half_rn(acc[e] * w_norm);
-                }
-                __syncwarp();
+            const bool taken = words[kTaken] == i + 1 || words[kTaken + 1] == i + 1 || words[kTaken + 2] == i + 1 || words[kTaken + 3] == i + 1;
+            if (taken && busy) {
+                if (cut) add_hidden<D, true>(p, i, pos, d0, dims, valid ? part_row : nullptr);
+                else add_hidden<D, false>(p, i, pos, d0, dims, valid ? dst : nullptr);
             }
             if (cut) {
                 if (valid && (paired_rows || s == 0))
@@ -689,11 +791,11 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                 named_bar_sync(9, 256);
                 if (tid == 0) {
                     const uint32_t done = atomicAdd(p.tickets + it.counter, 1u) + 1;
-                    words[2] = done == it.n_parts;
+                    words[kLast] = done == it.n_parts;
                     if (done == it.n_parts) p.tickets[it.counter] = 0;  // for the next launch
                 }
                 named_bar_sync(10, 256);
-                if (words[2]) {
+                if (words[kLast]) {
                     // the last piece of the unit: all partial results are in memory
                     __threadfence();
                     // a thread takes 16 dims of a row; everything a piece has for it is requested at once
@@ -732,7 +834,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                                                pack_f16x2(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack_f16x2(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
                     }
                 }
-                named_bar_sync(9, 256);  // words[2] and the partial rows are free again
+                named_bar_sync(9, 256);  // words[kLast] and the partial rows are free again
             }
         }
     }
@@ -916,7 +1018,6 @@ mf_status mf_paged_chunk_attention(MfContext *ctx, const MfChunkPlan *pl, const 
     ChunkParams p{};
     p.q = static_cast<const __half *>(a->q);
     p.out = static_cast<__half *>(a->out);
-    p.k_pool = static_cast<const __half *>(c->k_pool);
     p.v_pool = static_cast<const __half *>(c->v_pool);
     p.page_table = c->page_table;
     p.list = pl->d_list;

@@ -20,16 +20,20 @@ MF_RING_FN bool ring_uses(bool paired_rows, uint32_t n, uint32_t stream, uint32_
     if (paired_rows) return true;
     return (load / 4) * 2 + 1 < n ? (load & 1u) == stream : stream == 0;
 }
-// The V load of a stream's j-th tile, counted from the item's first load.
-MF_RING_FN uint32_t ring_v_load(bool paired_rows, uint32_t n, uint32_t stream, uint32_t j)
+// The tile (from the item's first) whose V the load is; n or more: a K load.
+MF_RING_FN uint32_t ring_v_tile(bool paired_rows, uint32_t n, uint32_t load)
 {
-    return paired_rows ? 2 * j + 1 : 4 * j + (2 * j + 1 < n ? 2 + stream : 1);
+    if (paired_rows) return load & 1u ? load / 2 : n;
+    const uint32_t t = (load / 4) * 2;
+    if (t + 1 < n) return load & 2u ? t + (load & 1u) : n;
+    return load & 1u ? t : n;
 }
 
 // A stream's way through the ring.  It waits for EVERY load in turn, also for those that the other stream uses: a slot's
 // barrier is waited for by parity, and a reader that leaves out a use cannot tell the use after it from the one before
 // (with an odd number of slots the uses of a slot alternate between the streams).  A load that only the other stream uses
-// is handed back as soon as it has landed, so that a slot is free after one arrival of each stream, whatever the form.
+// is handed back as soon as it has landed, so that a slot is free after one arrival of each stream, whatever the form (and
+// one of the warp that prepares V tiles, which goes through all loads, too).
 template <uint32_t kSlots>
 struct RingReader {
     uint32_t slot = 0, phase = 0;  // of the next load
@@ -59,6 +63,8 @@ struct RingReader {
         }
         load = 0;
     }
+    // The phase of the load that next() has returned.
+    MF_RING_FN uint32_t last_phase() const { return slot == 0 ? phase ^ 1 : phase; }
     MF_RING_FN void step()
     {
         ++load;

@@ -10,7 +10,7 @@ from pathlib import Path
 import pytest
 
 HEADER = Path(__file__).resolve().parent.parent / "test-burn_b200" / "csrc" / "chunk_ring.hpp"
-WAIT, PASS, USE_K, USE_V = range(4)
+WAIT, PASS, USE_K, USE_V, FIT = range(5)
 
 # A stream's steps in the order in which the kernel's issuing warp takes them: (what, slot, parity).
 SOURCE = r"""
@@ -29,7 +29,9 @@ template <uint32_t S> static uint32_t walk(uint32_t stream, uint32_t items, cons
         auto next = [&]() { return reader.next(rows[i] != 0, n, stream, landed, pass); };
         if (mine) put(2, next(), 0);
         for (uint32_t j = 0; j < mine; ++j) {
-            put(3, next(), 0);
+            const uint32_t v = next();
+            put(4, v, reader.last_phase());
+            put(3, v, 0);
             if (j + 1 < mine) put(2, next(), 0);
         }
         reader.finish(n, landed, pass);
@@ -40,7 +42,7 @@ extern "C" uint32_t ring_walk(uint32_t slots, uint32_t stream, uint32_t items, c
 {
     return slots == 5 ? walk<5>(stream, items, tiles, rows, out) : slots == 10 ? walk<10>(stream, items, tiles, rows, out) : 0;
 }
-extern "C" uint32_t v_load(uint32_t rows, uint32_t n, uint32_t stream, uint32_t j) { return ring_v_load(rows != 0, n, stream, j); }
+extern "C" uint32_t v_tile(uint32_t rows, uint32_t n, uint32_t load) { return ring_v_tile(rows != 0, n, load); }
 extern "C" uint32_t uses(uint32_t rows, uint32_t n, uint32_t stream, uint32_t load) { return ring_uses(rows != 0, n, stream, load); }
 """
 
@@ -58,9 +60,14 @@ def ring(tmp_path_factory):
 def steps(ring, slots, stream, items):
     n = (C.c_uint32 * len(items))(*[t for t, _ in items])
     rows = (C.c_uint32 * len(items))(*[int(r) for _, r in items])
-    out = (C.c_uint32 * (3 * 8 * (sum(t for t, _ in items) + 1)))()
+    out = (C.c_uint32 * (3 * 12 * (sum(t for t, _ in items) + 1)))()
     m = ring.ring_walk(slots, stream, len(items), n, rows, out)
     return [tuple(out[3 * i:3 * i + 3]) for i in range(m)]
+
+
+def v_loads(ring, n, rows, stream):
+    """The V loads that a stream uses, in order, counted from the item's first load."""
+    return [x for x in range(2 * n) if ring.v_tile(int(rows), n, x) < n and ring.uses(int(rows), n, stream, x)]
 
 
 def own_waits_only(slots, stream, items):
@@ -72,7 +79,7 @@ def own_waits_only(slots, stream, items):
             return 2 * t + v if rows else (4 * (t // 2) + (2 * v + t % 2 if t // 2 * 2 + 1 < n else v))
         def use(t, v):
             at = base + load(t, v)
-            return [(WAIT, at % slots, at // slots & 1), (USE_V if v else USE_K, at % slots, 0 if rows else 1)]
+            return [(WAIT, at % slots, at // slots & 1)] + [(FIT, at % slots, at // slots & 1)] * v + [(USE_V if v else USE_K, at % slots, 0 if rows else 1)]
         for j, t in enumerate(mine):
             if j == 0:
                 out += use(t, 0)
@@ -107,12 +114,12 @@ class EarlyWait(Exception):
 
 
 def simulate(ring, slots, items, walks, seed):
-    """Runs producer, two issuing warps, two softmax groups and the tensor pipe; raises EarlyWait when a wait returns before
+    """Runs producer, two issuing warps, the warp that prepares V tiles, two softmax groups and the tensor pipe; raises EarlyWait when a wait returns before
     the load it is for has landed, or when a load lands in a tile that is still read."""
     rng = random.Random(seed)
     slow = rng.choice([0.0, 0.1, 0.3])
     delay = lambda mean: rng.expovariate(1 / mean) * (rng.choice([1, 20]) if rng.random() < slow else 1)  # noqa: E731
-    full, empty = [Barrier(1) for _ in range(slots)], [Barrier(2) for _ in range(slots)]
+    full, empty = [Barrier(1) for _ in range(slots)], [Barrier(3) for _ in range(slots)]
     loads = 2 * sum(n for n, _ in items)
     landed, issued = [False] * loads, [False] * loads
     readers = [0] * loads
@@ -163,17 +170,17 @@ def simulate(ring, slots, items, walks, seed):
         if load + slots < loads and issued[load + slots]:
             raise EarlyWait(f"{who}: load {load} has been replaced")
 
-    # what the streams' uses are, in the order of their walks: (load, is V, number of the tile in the stream)
+    # what the streams' uses are, in the order of their walks: loads of K and V tiles; which V tiles need preparing
     def uses(stream):
         base = 0
         for n, rows in items:
-            mine = n if rows else (n + 1 - stream) // 2
-            for j in range(mine):
-                v = ring.v_load(int(rows), n, stream, j)
+            for j, v in enumerate(v_loads(ring, n, rows, stream)):
                 yield base + v - (2 if not rows and 2 * j + 1 < n else 1), base + v
             base += 2 * n
 
-    scores, weights = [Barrier(1) for _ in range(2)], [Barrier(1) for _ in range(2)]
+    prepared = {load for load in range(loads) if rng.random() < 0.4}
+
+    scores, weights, fit = [Barrier(1) for _ in range(2)], [Barrier(1) for _ in range(2)], [Barrier(1) for _ in range(slots)]
 
     def issuer(s, walk):
         mine = list(uses(s))
@@ -196,6 +203,12 @@ def simulate(ring, slots, items, walks, seed):
                 yield full[slot], extra
             elif what == PASS:
                 empty[slot].arrive(wake)
+            elif what == FIT:
+                load = order[at_use]
+                if load in prepared:
+                    yield fit[slot], extra
+                    if load not in ready:
+                        raise EarlyWait(f"stream {s}: load {load} has not been prepared")
             else:
                 load = order[at_use]
                 at_use += 1
@@ -219,16 +232,31 @@ def simulate(ring, slots, items, walks, seed):
                 yield delay(0.05)
         assert at_use == len(order)
 
+    ready = set()
+
+    def preparer():
+        base = 0
+        for n, rows in items:
+            for x in range(2 * n):
+                load = base + x
+                yield full[load % slots], load // slots & 1
+                check(load, "preparing")
+                if load in prepared and ring.v_tile(int(rows), n, x) < n:
+                    yield delay(0.2)
+                    check(load, "preparing")
+                    ready.add(load)
+                fit[load % slots].arrive(wake)
+                empty[load % slots].arrive(wake)
+            base += 2 * n
+
     def softmax(s):
-        for t, (_, v) in enumerate(list(uses(s))):
+        for t in range(len(list(uses(s)))):
             yield scores[s], t & 1
             yield delay(0.5)
-            if rng.random() < 0.7:  # a tile cut by a mask: its V rows are looked at
-                yield full[v % slots], v // slots & 1
-                check(v, f"softmax group {s}")
             weights[s].arrive(wake)
 
     run(producer())
+    run(preparer())
     for s in range(2):
         run(issuer(s, walks[s]))
         run(softmax(s))
@@ -236,7 +264,7 @@ def simulate(ring, slots, items, walks, seed):
         now, _, fn = heapq.heappop(events)
         fn()
     assert all(landed) and not any(readers), "the ring stood still"
-    assert [b.phase for b in empty] == [len(range(x, loads, slots)) for x in range(slots)] and all(b.left == 2 for b in empty)
+    assert [b.phase for b in empty] == [len(range(x, loads, slots)) for x in range(slots)] and all(b.left == 3 for b in empty)
 
 
 def items_of(rng, count, most):
@@ -253,8 +281,8 @@ def test_uses_of_an_item(ring, slots):
                 assert used == [1, 1] if rows else sum(used) == 1
             for s in range(2):
                 mine = n if rows else (n + 1 - s) // 2
-                v = [ring.v_load(rows, n, s, j) for j in range(mine)]
-                assert all(ring.uses(rows, n, s, x) for x in v) and v == sorted(set(v)) and all(x < 2 * n for x in v)
+                v = v_loads(ring, n, rows, s)
+                assert [ring.v_tile(rows, n, x) for x in v] == [j if rows else 2 * j + s for j in range(mine)]
                 walk = steps(ring, slots, s, [(n, rows)])
                 waits = [(slot, phase) for what, slot, phase in walk if what == WAIT]
                 assert waits == [(x % slots, x // slots & 1) for x in range(2 * n)]
