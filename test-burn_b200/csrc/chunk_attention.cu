@@ -22,8 +22,9 @@
 // [8-row group][half][8 rows][128 bytes], so the 128 rows of a tile are evenly spaced 8-row groups whatever the page
 // size, and both operands (K by rows, V by columns) take one descriptor per tile.
 //
-// O is rescaled only when a row's maximum has grown by more than 2^8 since the last rescale; weights are then at most
-// 256 and are rounded to f16 for the product (2^-11 of each), sums, maxima and accumulators are f32.
+// O is rescaled only when a row's maximum has grown by more than 2^8 since the last rescale.  Weights carry a constant
+// factor of 2^7 (it cancels in the division): at most 2^15, they are rounded to f16 for the product (2^-11 of each, 2^-32 of
+// the reference maximum below 2^-21 of it), sums, maxima and accumulators are f32.
 //
 // Rows of a tile that no row of the unit sees (the end of the cache, the edge of the window) are cleared in V: their
 // weight is zero, but zero times a stale NaN is not.  For the same reason elements that are not finite are taken out of the
@@ -86,7 +87,8 @@ constexpr uint32_t kThreads = 384;
 constexpr uint32_t kProducerWarp = 8, kIssuerWarp = 9, kQWarp = 11;
 constexpr uint64_t kWaitNs = 2000000000ull;  // bits of the status word: the `code` of the wait that ran out (kStatusBadPage is none of them)
 constexpr float kNegInf = -1e30f;
-constexpr float kRescaleThreshold = 8.0f;  // log2 of the largest weight kept in P
+constexpr float kRescaleThreshold = 8.0f;  // log2 of the largest growth of a row's maximum without a rescale
+constexpr float kWeightShift = 7.0f;       // log2 of the weight of the reference maximum: 2^(8 + 7) fits f16
 constexpr uint32_t kHalfTile = kTile * 128;
 
 __host__ __device__ constexpr uint32_t tile_bytes(uint32_t d) { return kTile * d * 2; }
@@ -650,7 +652,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                             }
                             tc_wait_st();
                         }
-                        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(-m_ref, -m_ref);
+                        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(kWeightShift - m_ref, kWeightShift - m_ref);
                         float2 acc_a = make_float2(0.f, 0.f), acc_b = make_float2(0.f, 0.f);
 #pragma unroll
                         for (uint32_t c = 0; c < N / 32; ++c) {
