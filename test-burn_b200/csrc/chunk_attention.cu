@@ -167,6 +167,14 @@ __device__ __forceinline__ uint32_t page_entry(const ChunkItem &it, uint32_t v)
 }
 __device__ __forceinline__ uint32_t low_bits(int32_t n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
 
+// 1 / the sum of a row's weights.  A row before the start of the cache sees nothing and comes out as zeros; any other sees
+// its own key at least: a sum of 0 means that all its scores are -inf, which is as little a number as a NaN among them.
+__device__ __forceinline__ float inverse_sum(float sum, int32_t pos)
+{
+    if (sum > 0.f) return 1.f / sum;
+    return pos < 0 ? 0.f : __int_as_float(0x7FFFFFFF);
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c)
 {
     float d;
@@ -702,7 +710,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             if (mine) o_phase ^= 1;
             tc_fence_after();
             const bool cut = it.n_parts > 1;
-            const float norm = cut ? 1.f : (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));  // a sum that is not a number shows
+            const float norm = cut ? 1.f : inverse_sum(l, pos);
             f0 *= norm;
             f1 *= norm;
             const uint32_t d0 = paired_rows ? 0 : s * (D / 2), dims = paired_rows ? D : D / 2;
@@ -826,8 +834,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                                 o[4 * e + 3] = fmaf(a[e].w, f, o[4 * e + 3] * f_old);
                             }
                         }
-                        const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
                         const uint32_t tk = row / G;
+                        const float inv = inverse_sum(sum, it.pos0 + (int32_t)tk);
                         uint4 *to = reinterpret_cast<uint4 *>(p.out + (it.tok0 + (uint64_t)tk) * p.out_stride_t +
                                                               (uint64_t)(it.kvh * G + row - tk * G) * p.out_stride_h + grp * 16);
 #pragma unroll

@@ -140,3 +140,38 @@ def test_a_value_that_is_not_finite_costs_no_time(mfk, foundry, value, q_lens, k
         assert torch.equal(got[~rows], want[~rows])
     assert bad <= 2 * clean + 0.05, f"{bad:.3f} ms with it, {clean:.3f} ms without"
     plan.close()
+
+
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+@pytest.mark.parametrize("q_lens,kv_lens,hq,hkv,d,window,sinks", [
+    ([1], [1], 8, 2, 128, 0, 0),
+    ([1, 1, 1], [1, 700, 5000], 8, 1, 64, 1, 0),
+    ([40, 7], [40, 300], 16, 2, 128, 0, 0),
+    ([200, 3], [900, 3], 14, 2, 64, 40, 2),
+    ([9], [4], 8, 2, 128, 0, 0),
+    ([1, 5], [20000, 30000], 8, 1, 128, 0, 0),
+])
+def test_keys_show_as_the_formula_has_them(mfk, foundry, value, q_lens, kv_lens, hq, hkv, d, window, sinks):
+    """A key that is not finite makes its score +inf, -inf or NaN: a NaN in the rows that see it, but for a score of -inf beside
+    finite ones, whose weight is 0; a row that sees nothing but -inf is not a number either."""
+    case = ChunkCase(hq=hq, hkv=hkv, d=d, page=16, q_lens=q_lens, kv_lens=kv_lens, window=window, sinks=sinks)
+    for b, n in enumerate(kv_lens):
+        for key in {n - 1, n // 2, 0}:
+            case.kc[b][:, key, 1] = value
+            put(case, b, key, [1], value, case.k)
+    got = run(mfk, foundry, case)
+    t = 0
+    for b, nq in enumerate(q_lens):
+        see = case.visible(b)
+        for h in range(hq):
+            k, v = case.kc[b][h // (hq // hkv)].double(), case.vc[b][h // (hq // hkv)].double()
+            s = (case.q[t:t + nq, h * d:(h + 1) * d].double() @ k.T * d ** -0.5).masked_fill(~see, -INF)
+            w = torch.softmax(s, -1)
+            w[~see.any(1)] = 0
+            want, mean = w @ v, w @ v.abs()
+            few = see.sum(1, keepdim=True) * 2.0 ** -32 * float(v.abs().max())
+            tol = 2.0 ** -25 + 2.0 ** -11 * want.abs() + (2.0 ** -11 + 2.0 ** -12) * mean + few
+            off = (got[t:t + nq, h] - want).abs()
+            assert bool((torch.isnan(got[t:t + nq, h]) == torch.isnan(want)).all()), (b, h)
+            assert bool(((off <= tol) | torch.isnan(want)).all()), (b, h)
+        t += nq
