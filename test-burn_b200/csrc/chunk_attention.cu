@@ -182,6 +182,36 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return d;
 }
 
+// Past 2^24 the rounding of a reference maximum alone is worth a factor of two and more.
+__device__ __forceinline__ bool is_far(float m_ref) { return fabsf(m_ref) > 16777216.f && m_ref > kNegInf; }
+
+// The weights of a half tile in which some row of the warp has a reference maximum so far from 0: it is subtracted before the
+// scaling.  Reads the scores from TMEM once more, writes the weights over them, returns their sum.
+__device__ __noinline__ float far_weights(uint32_t tm, const Visible vis, int32_t x0, bool valid, float m_ref, float m_raw, float scale)
+{
+    const bool far = is_far(m_ref);
+    const float sub = far ? m_raw : 0.f, shift = far ? kWeightShift : kWeightShift - m_ref;
+    float sum = 0.f;
+#pragma unroll 1
+    for (uint32_t c = 0; c < 2; ++c) {
+        const int32_t x = x0 + (int32_t)c * 32;
+        const uint32_t see = valid ? low_bits(vis.a - x) | (low_bits(vis.c - x) & ~low_bits(vis.b - x)) : 0xFFFFFFFFu;
+        uint32_t r[32], pk[16];
+        tmem_ld32(tm + c * 32, r);
+        tc_wait_ld();
+#pragma unroll
+        for (uint32_t q = 0; q < 32; ++q) {
+            const float w = (see >> q) & 1u ? fast_exp2(fmaf(__uint_as_float(r[q]) - sub, scale, shift)) : 0.f;
+            sum += w;
+            r[q] = __float_as_uint(w);
+        }
+#pragma unroll
+        for (uint32_t q = 0; q < 16; ++q) pk[q] = pack_f16x2(__uint_as_float(r[2 * q]), __uint_as_float(r[2 * q + 1]));
+        tmem_st16(tm + c * 16, pk);
+    }
+    return sum;
+}
+
 // Columns of a unit's page list by who sees them.  [gap0, gap1) and what lies behind `end`: no row.  [sink0, sink1),
 // [edge0, edge1), [diag0, diag1): some rows.  All others: every row.  (Rows only gain keys at the diagonal and lose keys at
 // the window's edge: the first and the last row have them all.)
@@ -600,7 +630,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             const Visible vis = visible(p, it, pos);
             const int32_t any_c = visible(p, it, it.pos0 + (int32_t)it.n_tok - 1).c;  // columns from here on: no row of the unit
             const uint32_t mine = paired_rows ? n : (n + 1 - s) / 2;
-            float m_ref = kNegInf, l = 0.f;
+            float m_ref = kNegInf, m_raw = 0.f, l = 0.f;  // the reference maximum, with and without the scale
+            bool far = false;  // some row of the warp has one far from 0
             for (uint32_t j = 0; j < mine; ++j) {
                 const uint32_t t = paired_rows ? j : 2 * j + s;
 #pragma unroll 1
@@ -641,44 +672,51 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                         const float m_new = mx > -3.0e38f ? mx * p.scale_log2 : kNegInf;
                         const bool grow = valid && m_new > m_ref + kRescaleThreshold;
                         const float m_old = m_ref;
-                        if (grow) m_ref = m_new;
-                        if ((j > 0 || h > 0) && __any_sync(0xffffffffu, grow)) {
-                            // O has to hold every earlier P V before it is scaled.  The one before the last has completed
-                            // (its half's scores were issued behind it), so the parity is unambiguous.
-                            wait(bar(kODone + s), (pv - 1) & 1, 16384u);
-                            tc_fence_after();
-                            const float alpha = fast_exp2(m_old - m_ref);
-                            l *= alpha;
+                        if (grow) m_ref = m_new, m_raw = mx;
+                        if (__any_sync(0xffffffffu, grow)) {
+                            if (j > 0 || h > 0) {
+                                // O has to hold every earlier P V before it is scaled.  The one before the last has completed
+                                // (its half's scores were issued behind it), so the parity is unambiguous.
+                                wait(bar(kODone + s), (pv - 1) & 1, 16384u);
+                                tc_fence_after();
+                                const float alpha = fast_exp2(m_old - m_ref);
+                                l *= alpha;
 #pragma unroll 1
-                            for (uint32_t c = 0; c < D / 32; ++c) {
-                                uint32_t ob[32];
-                                tmem_ld32(o_base + s * 128 + c * 32, ob);
-                                tc_wait_ld();
+                                for (uint32_t c = 0; c < D / 32; ++c) {
+                                    uint32_t ob[32];
+                                    tmem_ld32(o_base + s * 128 + c * 32, ob);
+                                    tc_wait_ld();
 #pragma unroll
-                                for (uint32_t q = 0; q < 32; ++q) ob[q] = __float_as_uint(__uint_as_float(ob[q]) * alpha);
-                                tmem_st32(o_base + s * 128 + c * 32, ob);
+                                    for (uint32_t q = 0; q < 32; ++q) ob[q] = __float_as_uint(__uint_as_float(ob[q]) * alpha);
+                                    tmem_st32(o_base + s * 128 + c * 32, ob);
+                                }
+                                tc_wait_st();
                             }
-                            tc_wait_st();
+                            far = __any_sync(0xffffffffu, is_far(m_ref));
                         }
-                        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(kWeightShift - m_ref, kWeightShift - m_ref);
-                        float2 acc_a = make_float2(0.f, 0.f), acc_b = make_float2(0.f, 0.f);
+                        if (far) {
+                            l += far_weights(sp_tm, vis, x0, valid, m_ref, m_raw, p.scale_log2);
+                        } else {
+                            const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(kWeightShift - m_ref, kWeightShift - m_ref);
+                            float2 acc_a = make_float2(0.f, 0.f), acc_b = make_float2(0.f, 0.f);
 #pragma unroll
-                        for (uint32_t c = 0; c < N / 32; ++c) {
-                            uint32_t pk[16];
+                            for (uint32_t c = 0; c < N / 32; ++c) {
+                                uint32_t pk[16];
 #pragma unroll
-                            for (uint32_t q = 0; q < 16; ++q) {
-                                const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c * 32 + 2 * q]), __uint_as_float(r[c * 32 + 2 * q + 1])), sc2, nm2);
-                                float2 w;
-                                w.x = fast_exp2(x.x);
-                                w.y = fast_exp2(x.y);
-                                if (q & 1) acc_b = __fadd2_rn(acc_b, w);
-                                else acc_a = __fadd2_rn(acc_a, w);
-                                pk[q] = pack_f16x2(w.x, w.y);
+                                for (uint32_t q = 0; q < 16; ++q) {
+                                    const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c * 32 + 2 * q]), __uint_as_float(r[c * 32 + 2 * q + 1])), sc2, nm2);
+                                    float2 w;
+                                    w.x = fast_exp2(x.x);
+                                    w.y = fast_exp2(x.y);
+                                    if (q & 1) acc_b = __fadd2_rn(acc_b, w);
+                                    else acc_a = __fadd2_rn(acc_a, w);
+                                    pk[q] = pack_f16x2(w.x, w.y);
+                                }
+                                tmem_st16(sp_tm + c * 16, pk);
                             }
-                            tmem_st16(sp_tm + c * 16, pk);
+                            const float2 acc = __fadd2_rn(acc_a, acc_b);
+                            l += acc.x + acc.y;
                         }
-                        const float2 acc = __fadd2_rn(acc_a, acc_b);
-                        l += acc.x + acc.y;
                     }
                     tc_wait_st();
                     tc_fence_before();

@@ -175,3 +175,23 @@ def test_keys_show_as_the_formula_has_them(mfk, foundry, value, q_lens, kv_lens,
             assert bool((torch.isnan(got[t:t + nq, h]) == torch.isnan(want)).all()), (b, h)
             assert bool(((off <= tol) | torch.isnan(want)).all()), (b, h)
         t += nq
+
+
+@pytest.mark.parametrize("size", [1.0, 250.0, 4000.0, 65504.0])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1], [4000]), ([60, 1], [300, 90])])
+def test_large_scores(mfk, foundry, size, q_lens, kv_lens):
+    """Equal scores up to those of f16's largest values, of either sign: every visible key has the same weight."""
+    for sign in (1.0, -1.0):
+        case = ChunkCase(hq=8, hkv=2, d=128, page=16, q_lens=q_lens, kv_lens=kv_lens)
+        case.q.fill_(size)
+        case.k[torch.isfinite(case.k)] = sign * size
+        got = run(mfk, foundry, case)
+        t = 0
+        for b, nq in enumerate(q_lens):
+            see = case.visible(b).double()
+            for h in range(8):
+                v = case.vc[b][h // 4].double()
+                want, mean = see @ v / see.sum(1, keepdim=True), see @ v.abs() / see.sum(1, keepdim=True)
+                tol = 2.0 ** -25 + 2.0 ** -11 * want.abs() + (2.0 ** -11 + 2.0 ** -12) * mean
+                assert bool(((got[t:t + nq, h] - want).abs() <= tol).all())
+            t += nq
