@@ -680,7 +680,7 @@ MF_API uint32_t mf_chunk_plan_build_host(const uint32_t *q_lens_host, const uint
                                          uint32_t n_sinks, uint32_t n_ctas, uint32_t *items_out, uint32_t item_capacity,
                                          uint32_t *cta_begin_out);
 /* q and out: f16, 16-byte aligned; element (token t, head h, dim d) at t * stride_t + h * stride_h + d,
- * strides in elements, multiples of 8; out does not overlap q.  q is rotated already.  scale >= 0. */
+ * strides in elements, multiples of 8; out does not overlap q.  q is rotated already.  scale: 0 to 1e18. */
 typedef struct MfPagedChunkArgs {
     const void *q;
     void *out;

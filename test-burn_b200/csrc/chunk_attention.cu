@@ -47,7 +47,6 @@
 //
 // TMEM columns (512): halves 0, 1 of S_0/P_0 [0,64) [64,128), of S_1/P_1 [128,192) [192,256), O_0 [256,384)  O_1 [384,512).
 #include <algorithm>
-#include <cmath>
 #include <cstring>
 #include <new>
 #include <vector>
@@ -86,7 +85,9 @@ constexpr uint32_t kTile = kChunkTile;
 constexpr uint32_t kThreads = 384;
 constexpr uint32_t kProducerWarp = 8, kIssuerWarp = 9, kQWarp = 11;
 constexpr uint64_t kWaitNs = 2000000000ull;  // bits of the status word: the `code` of the wait that ran out (kStatusBadPage is none of them)
-constexpr float kNegInf = -1e30f;
+constexpr float kNegInf = -1e30f;  // a row's maximum before its first key
+// Products of f16 rows of 128 are below 2^39: with this scale every finite score stays above kNegInf.
+constexpr float kMaxScale = 1e18f;
 constexpr float kRescaleThreshold = 8.0f;  // log2 of the largest growth of a row's maximum without a rescale
 constexpr float kWeightShift = 7.0f;       // log2 of the weight of the reference maximum: 2^(8 + 7) fits f16
 constexpr uint32_t kHalfTile = kTile * 128;
@@ -1059,7 +1060,7 @@ mf_status mf_paged_chunk_attention(MfContext *ctx, const MfChunkPlan *pl, const 
         return fail(ctx, MF_ERR_INVALID_SHAPE, "paged chunk attention: q, out and the pools must be 16-byte aligned");
     if ((a->q_stride_t | a->q_stride_h | a->out_stride_t | a->out_stride_h) & 7u)
         return fail(ctx, MF_ERR_INVALID_SHAPE, "paged chunk attention: strides must be multiples of 8 elements");
-    if (!(a->scale >= 0.f) || !std::isfinite(a->scale * 1.4426950408889634f))
+    if (!(a->scale >= 0.f && a->scale <= kMaxScale))
         return fail(ctx, MF_ERR_INVALID_OPERATION, "paged chunk attention: scale %g", (double)a->scale);
     if (pl->max_tokens == 0 || !a->q || !a->out) return MF_OK;
     DeviceScope scope(ctx->device);

@@ -177,6 +177,36 @@ def test_keys_show_as_the_formula_has_them(mfk, foundry, value, q_lens, kv_lens,
         t += nq
 
 
+def test_large_scales(mfk, foundry):
+    """With large scales the key of the largest score has all the weight; a scale whose scores would leave the range is refused."""
+    case = ChunkCase(hq=8, hkv=2, d=128, page=16, q_lens=[1, 40], kv_lens=[50, 300])
+    plan, out = case.plan(foundry), torch.empty_like(case.q)
+    t = 0
+    best = torch.zeros((case.tokens, 8, 128), dtype=torch.float16, device="cuda")
+    clear = torch.zeros((case.tokens, 8, 1), dtype=torch.bool, device="cuda")
+    for b, nq in enumerate(case.q_lens):
+        for h in range(8):
+            s = (case.q[t:t + nq, h * 128:(h + 1) * 128].double() @ case.kc[b][h // 4].double().T).masked_fill(~case.visible(b), -INF)
+            top = s.topk(2, 1).values
+            clear[t:t + nq, h, 0] = top[:, 0] - top[:, 1] > 2.0 ** -10  # (f32 products of up to 50: off by less than 2^-14)
+            best[t:t + nq, h] = case.vc[b][h // 4][s.argmax(1)]
+        t += nq
+    assert float(clear.float().mean()) > 0.95
+    for scale in (1e6, 1e12, 1e18):
+        foundry.paged_chunk_attention(plan, case.cache(mfk), case.q, out, scale=scale)
+        foundry.synchronize()
+        got = out.view_as(best)
+        assert torch.equal(got[clear.expand_as(got)], best[clear.expand_as(got)])
+    out.fill_(7.0)
+    for scale in (2e18, 1e30, 2e38):
+        with pytest.raises(mfk.MetalError) as e:
+            foundry.paged_chunk_attention(plan, case.cache(mfk), case.q, out, scale=scale)
+        assert e.value.kind == "InvalidOperation"
+    foundry.synchronize()
+    assert bool((out == 7.0).all())
+    plan.close()
+
+
 @pytest.mark.parametrize("size", [1.0, 250.0, 4000.0, 65504.0])
 @pytest.mark.parametrize("q_lens,kv_lens", [([1], [4000]), ([60, 1], [300, 90])])
 def test_large_scores(mfk, foundry, size, q_lens, kv_lens):
