@@ -913,6 +913,16 @@ mf_status check_lens(MfContext *ctx, const uint32_t *q_lens, const uint32_t *kv_
     return MF_OK;
 }
 
+mf_status refuse_in_capture(MfContext *ctx, const char *what)
+{
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    const mf_status st = check_cuda(ctx, cudaStreamIsCapturing(ctx->stream, &cap), "cudaStreamIsCapturing");
+    if (st != MF_OK) return st;
+    if (cap != cudaStreamCaptureStatusNone)
+        return fail(ctx, MF_ERR_INVALID_OPERATION, "chunk plan: %s while the stream is being captured", what);
+    return MF_OK;
+}
+
 }  // namespace
 }  // namespace mf
 
@@ -943,10 +953,7 @@ mf_status mf_chunk_plan_update(MfContext *ctx, MfChunkPlan *pl, const uint32_t *
     if (st != MF_OK) return st;
     if (tokens > pl->max_tokens)
         return fail(ctx, MF_ERR_INVALID_SHAPE, "chunk plan: %llu new tokens, made for %u", (unsigned long long)tokens, pl->max_tokens);
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    if ((st = check_cuda(ctx, cudaStreamIsCapturing(ctx->stream, &cap), "cudaStreamIsCapturing")) != MF_OK) return st;
-    if (cap != cudaStreamCaptureStatusNone)
-        return fail(ctx, MF_ERR_INVALID_OPERATION, "chunk plan: no update while the stream is being captured");
+    if ((st = refuse_in_capture(ctx, "no update")) != MF_OK) return st;
     try {
         build_chunk_plan(q_lens, kv_lens, pl->batch, pl->n_kv_heads, pl->n_heads / pl->n_kv_heads, pl->page_size, pl->window, pl->n_sinks,
                          pl->n_ctas, pl->h_items, pl->h_begin);
@@ -996,6 +1003,8 @@ mf_status mf_chunk_plan_create(MfContext *ctx, const uint32_t *q_lens, const uin
     if (st != MF_OK) return st;
     if (max_tokens > kMaxLen) return fail(ctx, MF_ERR_INVALID_SHAPE, "chunk plan: max_tokens %u", max_tokens);
     DeviceScope scope(ctx->device);
+    // (an allocation would end the capture with an error)
+    if ((st = refuse_in_capture(ctx, "no plan is made")) != MF_OK) return st;
     MfChunkPlan *pl = new (std::nothrow) MfChunkPlan();
     if (!pl) return fail(ctx, MF_ERR_OUT_OF_MEMORY, "chunk plan");
     pl->batch = batch;
