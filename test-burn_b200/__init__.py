@@ -264,6 +264,7 @@ _SIGNATURES = {
     "mf_prefix_cache_lookup": (C.c_int32, [vp, vp, u32, C.c_char_p, C.POINTER(u32), vp, u32, C.POINTER(u32)]),
     "mf_paged_prefill": (C.c_int32, [vp, C.POINTER(MfPagedKv), C.POINTER(MfPagedPrefillArgs)]),
     "mf_paged_copy_pages": (C.c_int32, [vp, C.POINTER(MfPagedKv), vp, vp, u32]),
+    "mf_is_capturing": (u32, [vp]),
     "mf_chunk_plan_create": (C.c_int32, [vp, vp, vp] + [u32] * 8 + [C.POINTER(vp)]),
     "mf_chunk_plan_update": (C.c_int32, [vp, vp, vp, vp]),
     "mf_chunk_plan_destroy": (None, [vp, vp]),
@@ -554,10 +555,14 @@ class Foundry:
 
     def paged_chunk_attention(self, plan: "ChunkPlan", cache: MfPagedKv, q, out, *, scale=None):
         """Causal (windowed) attention of the plan's new tokens; q and out: f16 [tokens, Hq*D] or [tokens, Hq, D], any
-        token and head strides that are multiples of 8."""
+        token and head strides that are multiples of 8.  A call that is captured into a CUDA graph follows later updates
+        of the plan, so its q and out have to hold the plan's max_tokens."""
         d = cache.head_dim
         qt, qh = _head_strides(q, plan, d, "q", self.device)
         ot, oh = _head_strides(out, plan, d, "out", self.device)
+        if (q.shape[0] < plan.max_tokens or out.shape[0] < plan.max_tokens) and lib.mf_is_capturing(self._h):
+            raise MetalError(2, f"paged chunk attention: q of {q.shape[0]} and out of {out.shape[0]} tokens in a captured call "
+                                f"whose plan may come to hold {plan.max_tokens}")
         a = _CHUNK_ARGS.pack(q.data_ptr(), out.data_ptr(), qt, qh, ot, oh, d ** -0.5 if scale is None else scale)
         self.check(lib.mf_paged_chunk_attention(self._h, plan._h, C.byref(cache), a))
 
@@ -889,6 +894,7 @@ class ChunkPlan:
                                                head_dim, page_size, window, sinks, max_tokens, C.byref(h)))
         self._h = h
         self.tokens = int(ql.sum())
+        self.max_tokens = max_tokens or self.tokens
 
     @staticmethod
     def _lens(q_lens, kv_lens):

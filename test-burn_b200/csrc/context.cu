@@ -269,6 +269,12 @@ mf_status mf_context_set_scratch(MfContext *ctx, void *dev_ptr, uint64_t bytes)
     return MF_OK;
 }
 
+uint32_t mf_is_capturing(const MfContext *ctx)
+{
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    return ctx && cudaStreamIsCapturing(ctx->stream, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone ? 1u : 0u;
+}
+
 mf_status mf_context_set_option(MfContext *ctx, uint32_t option, uint32_t value)
 {
     if (!ctx) return MF_ERR_INPUT_NOT_FOUND;
