@@ -1025,9 +1025,10 @@ mf_status mf_chunk_plan_create(MfContext *ctx, const uint32_t *q_lens, const uin
     pl->item_capacity = chunk_item_capacity(batch, pl->max_tokens, n_kv_heads, n_heads / n_kv_heads, pl->n_ctas);
     const size_t list_bytes = (4 * (size_t)pl->begin_words + pl->item_capacity * sizeof(ChunkItem) + 255) / 256 * 256;
     const size_t rows = (size_t)chunk_slots(pl->n_ctas) * 2 * kTile, acc_bytes = rows * head_dim * 4, ml_bytes = rows * 8;
-    ok(cudaMallocHost(reinterpret_cast<void **>(&pl->pinned[0]), 2 * list_bytes));
-    for (int i = 0; i < 2; ++i) ok(cudaEventCreateWithFlags(&pl->staged[i], cudaEventDisableTiming));
+    // the GPU's memory first: what it cannot hold is not asked of the host, twice as large and pinned
     ok(cudaMalloc(&pl->device_block, acc_bytes + ml_bytes + list_bytes + 4 * (size_t)pl->n_ctas));
+    if (e == cudaSuccess) ok(cudaMallocHost(reinterpret_cast<void **>(&pl->pinned[0]), 2 * list_bytes));
+    for (int i = 0; i < 2 && e == cudaSuccess; ++i) ok(cudaEventCreateWithFlags(&pl->staged[i], cudaEventDisableTiming));
     if (e == cudaSuccess) {
         char *at = static_cast<char *>(pl->device_block);
         pl->pinned[1] = pl->pinned[0] + list_bytes / 4;
@@ -1037,7 +1038,7 @@ mf_status mf_chunk_plan_create(MfContext *ctx, const uint32_t *q_lens, const uin
         pl->d_tickets = reinterpret_cast<uint32_t *>(at + acc_bytes + ml_bytes + list_bytes);
     }
     // (here rather than at the first launch, which may be inside a stream capture)
-    ok(cudaFuncSetAttribute(chunk_kernel(head_dim), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(head_dim)));
+    if (e == cudaSuccess) ok(cudaFuncSetAttribute(chunk_kernel(head_dim), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(head_dim)));
     st = e == cudaSuccess ? mf_chunk_plan_update(ctx, pl, q_lens, kv_lens) : check_cuda(ctx, e, "chunk plan allocation");
     if (st != MF_OK) {
         mf_chunk_plan_destroy(ctx, pl);

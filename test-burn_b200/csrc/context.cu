@@ -28,6 +28,7 @@ mf_status fail(MfContext *ctx, mf_status code, const char *fmt, ...)
 mf_status check_cuda(MfContext *ctx, cudaError_t e, const char *what)
 {
     if (e == cudaSuccess) return MF_OK;
+    (void)cudaGetLastError();  // reported here: the next launch's check must not find it again
     return fail(ctx, e == cudaErrorMemoryAllocation ? MF_ERR_OUT_OF_MEMORY : MF_ERR_CUDA, "%s: %s", what,
                 cudaGetErrorString(e));
 }

@@ -1,4 +1,4 @@
-"""GPU: plans of ragged batches and stream capture: what a capture cannot hold is refused and leaves the capture as it was."""
+"""GPU: plans of ragged batches, stream capture and memory: what cannot be is refused and leaves everything as it was."""
 import pytest
 import torch
 
@@ -57,3 +57,16 @@ def test_a_captured_call_has_room_for_later_updates(mfk):
     del graph
     plan.close()
     f.close()
+
+
+def test_a_plan_that_does_not_fit_leaves_nothing_behind(mfk, foundry):
+    """More work items than the GPU's memory holds (some 258 GB): refused, and the next call is not blamed for it."""
+    with pytest.raises(mfk.MetalError) as e:
+        foundry.chunk_plan([1], [1], n_heads=960, n_kv_heads=960, head_dim=64, page_size=16, max_tokens=1 << 30)
+    assert e.value.kind == "OutOfMemory"
+    case = ChunkCase(hq=8, hkv=2, d=128, page=16, q_lens=[3, 1], kv_lens=[100, 50])
+    plan, out = case.plan(foundry), torch.zeros_like(case.q)
+    foundry.paged_chunk_attention(plan, case.cache(mfk), case.q, out)
+    foundry.synchronize()
+    check(out, case)
+    plan.close()
