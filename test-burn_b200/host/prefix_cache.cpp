@@ -256,10 +256,21 @@ mf_status mf_page_pool_release_hidden(MfPagePool *pool, uint32_t *ids, uint32_t 
     const uint64_t first_seen = (uint64_t)kv_len - window + 1;
     const uint64_t lo = ((uint64_t)n_sinks + page_size - 1) / page_size;
     const uint64_t hi = first_seen / page_size < n ? first_seen / page_size : n;
+    // One reference per entry: a page that is listed more often than it has owners is noticed when they run out, and what
+    // was counted down until then is counted up again.
+    for (uint64_t i = lo; i < hi; ++i) {
+        if (ids[i] == UINT32_MAX) continue;
+        if (ids[i] >= pool->refs.size() || pool->refs[ids[i]] == 0) {
+            for (uint64_t j = lo; j < i; ++j)
+                if (ids[j] != UINT32_MAX) ++pool->refs[ids[j]];
+            return MF_ERR_INVALID_OPERATION;
+        }
+        --pool->refs[ids[i]];
+    }
     for (uint64_t i = lo; i < hi; ++i)
-        if (ids[i] != UINT32_MAX && (ids[i] >= pool->refs.size() || pool->refs[ids[i]] == 0)) return MF_ERR_INVALID_OPERATION;
+        if (ids[i] != UINT32_MAX) ++pool->refs[ids[i]];
     for (uint64_t i = lo; i < hi; ++i)
-        if (ids[i] != UINT32_MAX && pool->refs[ids[i]] > 0) {
+        if (ids[i] != UINT32_MAX) {
             release_pages(pool, &ids[i], 1);
             ids[i] = UINT32_MAX;
             ++*released;
