@@ -1002,6 +1002,8 @@ mf_status mf_chunk_plan_create(MfContext *ctx, const uint32_t *q_lens, const uin
     mf_status st = check_lens(ctx, q_lens, kv_lens, batch, &tokens, &max_kv);
     if (st != MF_OK) return st;
     if (max_tokens > kMaxLen) return fail(ctx, MF_ERR_INVALID_SHAPE, "chunk plan: max_tokens %u", max_tokens);
+    if (chunk_item_capacity(batch, max_tokens ? max_tokens : tokens, n_kv_heads, n_heads / n_kv_heads, (uint32_t)ctx->sm_count) > UINT32_MAX)
+        return fail(ctx, MF_ERR_INVALID_SHAPE, "chunk plan: %llu tokens of %u kv heads", (unsigned long long)(max_tokens ? max_tokens : tokens), n_kv_heads);
     DeviceScope scope(ctx->device);
     // (an allocation would end the capture with an error)
     if ((st = refuse_in_capture(ctx, "no plan is made")) != MF_OK) return st;

@@ -27,7 +27,8 @@ struct ChunkItem {
 };
 static_assert(sizeof(ChunkItem) == 64, "one item is four 16-byte loads");
 
-// Most items a step of max_tokens new tokens can have.
+constexpr uint32_t kChunkMaxCtas = 1u << 16;
+// Most items a step of max_tokens new tokens can have.  Items are numbered in 32 bits.
 uint64_t chunk_item_capacity(uint32_t batch, uint64_t max_tokens, uint32_t n_kv_heads, uint32_t group, uint32_t n_ctas);
 // Partial slots and tickets: a boundary between two CTAs cuts at most one unit.
 inline uint32_t chunk_slots(uint32_t n_ctas) { return 2 * n_ctas; }

@@ -170,10 +170,14 @@ extern "C" uint32_t mf_chunk_plan_build_host(const uint32_t *q_lens, const uint3
                                              uint32_t n_ctas, uint32_t *items_out, uint32_t item_capacity, uint32_t *cta_begin_out)
 {
     if (!q_lens || !kv_lens || !cta_begin_out || n_kv_heads == 0 || n_heads % n_kv_heads || n_heads / n_kv_heads == 0 ||
-        n_heads / n_kv_heads > 64 || page_size == 0 || n_ctas == 0)
+        n_heads / n_kv_heads > 64 || page_size == 0 || n_ctas == 0 || n_ctas > mf::kChunkMaxCtas)
         return 0;
-    for (uint32_t b = 0; b < batch; ++b)
+    uint64_t tokens = 0;
+    for (uint32_t b = 0; b < batch; ++b) {
         if (q_lens[b] > mf::kChunkMaxLen || kv_lens[b] > mf::kChunkMaxLen) return 0;
+        tokens += q_lens[b];
+    }
+    if (tokens > mf::kChunkMaxLen || mf::chunk_item_capacity(batch, tokens, n_kv_heads, n_heads / n_kv_heads, n_ctas) > UINT32_MAX) return 0;
     try {
         std::vector<mf::ChunkItem> items;
         std::vector<uint32_t> begin;

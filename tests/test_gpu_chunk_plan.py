@@ -70,3 +70,9 @@ def test_a_plan_that_does_not_fit_leaves_nothing_behind(mfk, foundry):
     foundry.synchronize()
     check(out, case)
     plan.close()
+
+
+def test_more_items_than_can_be_numbered(mfk, foundry):
+    with pytest.raises(mfk.MetalError) as e:
+        foundry.chunk_plan([1], [1], n_heads=4096, n_kv_heads=4096, head_dim=64, page_size=16, max_tokens=1 << 30)
+    assert e.value.kind == "InvalidShape"
