@@ -244,7 +244,9 @@ MF_API uint64_t mf_launch_count(const MfContext *ctx);
  * which bounds that set by the launch protocol alone), keeps the caches those launches write
  * and does not stream early from one of them (a one-layer model, or two calls in a row on one
  * cache); kernels of other origins that release their dependents early are the caller's to
- * vouch for.  Everything else a launch reads or writes still waits for the previous kernel.
+ * vouch for.  mf_paged_move_pages, mf_paged_mrope_append and their 8-bit forms may stand directly in front
+ * of a fused launch on the pools that they write: the launch then waits for them (mf_paged_kv_append,
+ * mf_paged_kv8_append and mf_paged_copy_pages may not, that is part of the promise).  Everything else a launch reads or writes still waits for the previous kernel.
  * Value 2 extends the early streaming to launches WITHOUT a fused append (the shards of a
  * sequence-sharded step that do not own the tail page): the caller then also promises that no
  * separate append kernel precedes the launch in the stream.

@@ -1121,7 +1121,9 @@ mf_status mf_paged_chunk_attention(MfContext *ctx, const MfChunkPlan *pl, const 
     auto *kern = chunk_kernel(c->head_dim);
     const uint32_t smem = smem_bytes(c->head_dim);
     kern<<<pl->n_ctas, kThreads, smem, ctx->stream>>>(tm_k, tm_v, tm_q, tm_q1, p);
-    return check_launch(ctx, "chunk_tc_kernel");
+    st = check_launch(ctx, "chunk_tc_kernel");
+    if (st == MF_OK) ctx->note_plain_launch(false);
+    return st;
 }
 
 }  // extern "C"

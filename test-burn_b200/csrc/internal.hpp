@@ -175,21 +175,33 @@ struct MfContext {
     const void *inflight_k[kWindow] = {}, *inflight_v[kWindow] = {};
     int n_inflight = 0;      // entries of the list
     int since_strict = 0;    // launches with the attribute after the last strict one
+    // The last launch without the attribute writes pools of its own choice (page moves, the multi-axis append), and no strict
+    // launch has waited for it yet: nothing streams early, and the next launch with the attribute is strict.
+    bool plain_writer = false;
     bool may_stream_early(const void *k_cache, const void *v_cache) const
     {
+        if (plain_writer) return false;
         for (int i = 0; i < n_inflight; ++i)
             if (k_cache == inflight_k[i] || k_cache == inflight_v[i] || v_cache == inflight_k[i] || v_cache == inflight_v[i])
                 return false;
         return true;
     }
     // Whether the next launch with the attribute has to be strict.
-    bool next_launch_strict() const { return since_strict + 1 >= kWindow; }
+    bool next_launch_strict() const { return plain_writer || since_strict + 1 >= kWindow; }
+    // After a launch without the attribute succeeded: it alone can be in flight now.
+    void note_plain_launch(bool writes_pools)
+    {
+        plain_writer = writes_pools;
+        n_inflight = 0;
+        since_strict = 0;
+    }
     // After such a launch succeeded; k_cache / v_cache: what it writes (null: no cache).
     void note_programmatic_launch(bool strict, const void *k_cache, const void *v_cache)
     {
         if (strict) {
             n_inflight = 0;
             since_strict = 0;
+            plain_writer = false;
         } else {
             ++since_strict;
         }

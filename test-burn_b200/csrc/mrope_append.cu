@@ -300,7 +300,9 @@ mf_status launch_mrope(MfContext *ctx, MropeParams &p, const char *what)
     const dim3 grid((uint32_t)blocks, (uint32_t)parts);
     if (p.head_dim == 128) mrope_append_kernel<128, K8><<<grid, kThreads, 0, ctx->stream>>>(p);
     else if constexpr (!K8) mrope_append_kernel<64, false><<<grid, kThreads, 0, ctx->stream>>>(p);
-    return check_launch(ctx, "mrope_append_kernel");
+    const mf_status st = check_launch(ctx, "mrope_append_kernel");
+    if (st == MF_OK) ctx->note_plain_launch(true);
+    return st;
 }
 
 }  // namespace

@@ -82,7 +82,9 @@ mf_status launch_moves(MfContext *ctx, const PoolRef *pools, uint32_t n_pools, c
         segments += (uint64_t)(k ? n_pools - p.n_wide : p.n_wide) * n * ((p.units[k] + kSegment - 1) / kSegment);
     const uint32_t blocks = (uint32_t)std::min<uint64_t>((segments + 7) / 8, (uint64_t)std::max(1, ctx->sm_count) * 8);
     move_pages_kernel<PAIRS><<<blocks, 256, 0, ctx->stream>>>(p);
-    return check_launch(ctx, "move_pages_kernel");
+    const mf_status st = check_launch(ctx, "move_pages_kernel");
+    if (st == MF_OK) ctx->note_plain_launch(true);
+    return st;
 }
 
 // pools: at most two page sizes, those of one size together.
