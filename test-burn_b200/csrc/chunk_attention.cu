@@ -946,6 +946,7 @@ mf_status mf_chunk_plan_update(MfContext *ctx, MfChunkPlan *pl, const uint32_t *
 {
     if (!ctx) return MF_ERR_INPUT_NOT_FOUND;
     if (!pl || !q_lens || !kv_lens) return fail(ctx, MF_ERR_INPUT_NOT_FOUND, "chunk plan: null input");
+    if (pl->device != ctx->device) return fail(ctx, MF_ERR_INVALID_OPERATION, "chunk plan: the plan is another device's");
     DeviceScope scope(ctx->device);
     uint64_t tokens;
     uint32_t max_kv;
