@@ -660,12 +660,14 @@ MF_API mf_status mf_paged_gather(MfContext *ctx, const MfPagedKv *cache, uint32_
  * A plan holds the lengths, the work list and the scratch of one such step; it is made from host
  * lengths, is reused by every layer with this geometry and this window, and is updated in place for
  * the next step.  max_tokens: the most new tokens of a later update (0: no more than now); the plan
- * allocates at creation only.  Updates are enqueued on the context's stream; launches that use one
- * plan must not overlap on the GPU (its partial results and tickets are shared by them), whether
- * eager or replayed.  A launch captured into a CUDA graph follows the updates made before its
+ * allocates at creation only.  Updates are enqueued on the context's stream; a launch on another
+ * stream waits for the last update, and the next update for it (not when it is captured).  Launches
+ * that use one plan must not overlap on the GPU (its partial results and tickets are shared by them),
+ * whether eager or replayed.  A launch captured into a CUDA graph follows the updates made before its
  * replay (q and out then have to hold max_tokens); making a plan and updating one are refused while
- * the stream is being captured, and a plan is destroyed when no capture is under way.  A plan takes 39 MB on the device at head_dim 128 (the partial results of units that
- * several CTAs share), half of that at 64, and 64 bytes per work item. */
+ * the stream is being captured, and a plan is destroyed when no capture is under way.  A plan takes
+ * 39 MB on the device at head_dim 128 (the partial results of units that several CTAs share), half of
+ * that at 64, and 64 bytes per work item. */
 typedef struct MfChunkPlan MfChunkPlan;
 MF_API mf_status mf_chunk_plan_create(MfContext *ctx, const uint32_t *q_lens_host, const uint32_t *kv_lens_host,
                                       uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,

@@ -74,6 +74,11 @@ struct MfChunkPlan {
     uint32_t next_stage = 0;
     float *d_acc = nullptr, *d_ml = nullptr;  // partial results: [slot][D / 4][256 rows][4], [slot][256 rows][2]
     uint32_t *d_tickets = nullptr;
+    // Launches on another stream than the last update's wait for its upload, and the next update waits for them.
+    cudaStream_t updated_on = nullptr;
+    cudaEvent_t used = nullptr;
+    mutable bool used_elsewhere = false;
+    bool updated = false;  // an update has been made
 };
 
 namespace mf {
@@ -935,8 +940,10 @@ void mf_chunk_plan_destroy(MfContext *ctx, MfChunkPlan *pl)
     if (!pl) return;
     DeviceScope scope(pl->device);
     if (ctx) cudaStreamSynchronize(ctx->stream);
+    if (pl->used_elsewhere) cudaEventSynchronize(pl->used);
     for (int i = 0; i < 2; ++i)
         if (pl->staged[i]) cudaEventDestroy(pl->staged[i]);
+    if (pl->used) cudaEventDestroy(pl->used);
     if (pl->pinned[0]) cudaFreeHost(pl->pinned[0]);
     if (pl->device_block) cudaFree(pl->device_block);
     delete pl;
@@ -966,6 +973,12 @@ mf_status mf_chunk_plan_update(MfContext *ctx, MfChunkPlan *pl, const uint32_t *
     const uint32_t s = pl->next_stage;
     if ((st = check_cuda(ctx, cudaEventSynchronize(pl->staged[s]), "chunk plan: staging")) != MF_OK) return st;
     uint32_t *w = pl->pinned[s];
+    if (pl->used_elsewhere && (st = check_cuda(ctx, cudaStreamWaitEvent(ctx->stream, pl->used, 0), "chunk plan: order")) != MF_OK) return st;
+    pl->used_elsewhere = false;
+    // (a second update from another stream follows the first)
+    if (pl->updated && pl->updated_on != ctx->stream &&
+        (st = check_cuda(ctx, cudaStreamWaitEvent(ctx->stream, pl->staged[s ^ 1], 0), "chunk plan: order")) != MF_OK)
+        return st;
     const size_t item_bytes = pl->h_items.size() * sizeof(ChunkItem);
     memcpy(w, pl->h_begin.data(), 4 * pl->h_begin.size());
     w[pl->begin_words - 1] = (uint32_t)tokens;
@@ -977,6 +990,8 @@ mf_status mf_chunk_plan_update(MfContext *ctx, MfChunkPlan *pl, const uint32_t *
     if ((st = check_cuda(ctx, cudaMemsetAsync(pl->d_tickets, 0, 4 * (size_t)pl->n_ctas, ctx->stream), "chunk plan: tickets")) != MF_OK) return st;
     if ((st = check_cuda(ctx, cudaEventRecord(pl->staged[s], ctx->stream), "chunk plan: upload")) != MF_OK) return st;
     pl->next_stage = s ^ 1;
+    pl->updated_on = ctx->stream;
+    pl->updated = true;
     pl->tokens = (uint32_t)tokens;
     pl->max_pages = (max_kv + pl->page_size - 1) / pl->page_size;
     return MF_OK;
@@ -1031,7 +1046,8 @@ mf_status mf_chunk_plan_create(MfContext *ctx, const uint32_t *q_lens, const uin
     // the GPU's memory first: what it cannot hold is not asked of the host, twice as large and pinned
     ok(cudaMalloc(&pl->device_block, acc_bytes + ml_bytes + list_bytes + 4 * (size_t)pl->n_ctas));
     if (e == cudaSuccess) ok(cudaMallocHost(reinterpret_cast<void **>(&pl->pinned[0]), 2 * list_bytes));
-    for (int i = 0; i < 2 && e == cudaSuccess; ++i) ok(cudaEventCreateWithFlags(&pl->staged[i], cudaEventDisableTiming));
+    for (cudaEvent_t *event : {&pl->staged[0], &pl->staged[1], &pl->used})
+        if (e == cudaSuccess) ok(cudaEventCreateWithFlags(event, cudaEventDisableTiming));
     if (e == cudaSuccess) {
         char *at = static_cast<char *>(pl->device_block);
         pl->pinned[1] = pl->pinned[0] + list_bytes / 4;
@@ -1119,12 +1135,24 @@ mf_status mf_paged_chunk_attention(MfContext *ctx, const MfChunkPlan *pl, const 
         if (st != MF_OK) return st;
         if (ok && ok1) p.q_tokens = pl->tokens;
     }
+    // A captured launch is not ordered here: it follows the plan as it stands at the replay.
+    const bool elsewhere = pl->updated_on != ctx->stream && !mf_is_capturing(ctx);
+    if (elsewhere) {
+        if ((st = check_cuda(ctx, cudaStreamWaitEvent(ctx->stream, pl->staged[pl->next_stage ^ 1], 0), "chunk plan: order")) != MF_OK) return st;
+        // (the event below stands for all such launches: a second stream's follow the first's)
+        if (pl->used_elsewhere && (st = check_cuda(ctx, cudaStreamWaitEvent(ctx->stream, pl->used, 0), "chunk plan: order")) != MF_OK) return st;
+    }
     auto *kern = chunk_kernel(c->head_dim);
     const uint32_t smem = smem_bytes(c->head_dim);
     kern<<<pl->n_ctas, kThreads, smem, ctx->stream>>>(tm_k, tm_v, tm_q, tm_q1, p);
     st = check_launch(ctx, "chunk_tc_kernel");
-    if (st == MF_OK) ctx->note_plain_launch(false);
-    return st;
+    if (st != MF_OK) return st;
+    ctx->note_plain_launch(false);
+    if (elsewhere) {
+        if ((st = check_cuda(ctx, cudaEventRecord(pl->used, ctx->stream), "chunk plan: order")) != MF_OK) return st;
+        pl->used_elsewhere = true;
+    }
+    return MF_OK;
 }
 
 }  // extern "C"

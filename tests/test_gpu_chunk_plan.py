@@ -76,3 +76,40 @@ def test_more_items_than_can_be_numbered(mfk, foundry):
     with pytest.raises(mfk.MetalError) as e:
         foundry.chunk_plan([1], [1], n_heads=4096, n_kv_heads=4096, head_dim=64, page_size=16, max_tokens=1 << 30)
     assert e.value.kind == "InvalidShape"
+
+
+def test_a_plan_on_another_stream_than_its_updates(mfk):
+    """A launch of another context waits for the update in front of it, and the next update waits for the launch, however late
+    either stream is."""
+    late = [torch.cuda.Stream() for _ in range(2)]
+    a, b = (mfk.Foundry(0, s.cuda_stream) for s in late)
+    kw = dict(hq=8, hkv=2, d=128, page=16)
+    cases = [ChunkCase(**kw, q_lens=q, kv_lens=kv, seed=i) for i, (q, kv) in
+             enumerate((([1, 1], [3000, 2000]), ([200, 3], [900, 3]), ([2, 190], [5, 700])))]
+    caches = [c.cache(mfk) for c in cases]
+    outs = [torch.zeros((256, 1024), dtype=torch.float16, device="cuda") for _ in cases]
+    qs = [torch.zeros((256, 1024), dtype=torch.float16, device="cuda") for _ in cases]
+    for q, c in zip(qs, cases):
+        q[:c.tokens] = c.q
+    plan = cases[0].plan(a, max_tokens=256)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(late[0]):
+            torch.cuda._sleep(3_000_000)
+        plan.update(cases[1].q_lens, cases[1].kv_lens)      # late, on a's stream
+        b.paged_chunk_attention(plan, caches[1], qs[1], outs[1])
+        with torch.cuda.stream(late[1]):
+            torch.cuda._sleep(3_000_000)
+        b.paged_chunk_attention(plan, caches[1], qs[1], outs[1])
+        plan.update(cases[2].q_lens, cases[2].kv_lens)      # not before b's launches are over
+        a.paged_chunk_attention(plan, caches[2], qs[2], outs[2])
+        a.synchronize()
+        b.synchronize()
+        for out, case in list(zip(outs, cases))[1:]:
+            check(out[:case.tokens], case)
+            assert not bool(out[case.tokens:].any())
+            out.zero_()
+        torch.cuda.synchronize()
+    plan.close()
+    a.close()
+    b.close()
