@@ -225,7 +225,7 @@ MF_API mf_status mf_context_create(int32_t device, void *cuda_stream, MfContext 
 MF_API void mf_context_destroy(MfContext *ctx);
 MF_API mf_status mf_context_set_stream(MfContext *ctx, void *cuda_stream);
 MF_API mf_status mf_synchronize(MfContext *ctx); /* Foundry::synchronize (lib.rs:170-188) */
-/* 1 while the context's stream is being captured into a CUDA graph, else 0. */
+/* 1 while the context's stream is being captured into a CUDA graph (or cannot be used because of a capture), else 0. */
 MF_API uint32_t mf_is_capturing(const MfContext *ctx);
 MF_API const char *mf_last_error(const MfContext *ctx);
 MF_API const char *mf_status_name(mf_status s);

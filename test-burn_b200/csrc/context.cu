@@ -273,7 +273,12 @@ mf_status mf_context_set_scratch(MfContext *ctx, void *dev_ptr, uint64_t bytes)
 uint32_t mf_is_capturing(const MfContext *ctx)
 {
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    return ctx && cudaStreamIsCapturing(ctx->stream, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone ? 1u : 0u;
+    if (!ctx) return 0;
+    if (cudaStreamIsCapturing(ctx->stream, &cap) != cudaSuccess) {
+        (void)cudaGetLastError();  // a refused query is an answer (the default stream while another one is being captured)
+        return 1;
+    }
+    return cap != cudaStreamCaptureStatusNone ? 1u : 0u;
 }
 
 mf_status mf_context_set_option(MfContext *ctx, uint32_t option, uint32_t value)

@@ -19,3 +19,7 @@ def test_refused(mfk, batch, q_len, hq, hkv, n_ctas):
 def test_most_ctas(mfk):
     items, begin = mfk.build_chunk_plan_host([40, 1], [300, 7000], n_heads=8, n_kv_heads=2, page_size=16, n_ctas=1 << 16)
     assert len(items) and begin[-1] == len(items)
+
+
+def test_no_context_is_not_being_captured(mfk):
+    assert mfk.lib.mf_is_capturing(None) == 0
