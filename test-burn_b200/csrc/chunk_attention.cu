@@ -34,16 +34,15 @@
 // (done by the groups it is 53 instead of 44 us for a prompt step of 14/2 heads of 64, window 512).
 //
 // What bounds it (measured on a B200):
-//   long prompts (6.8k new tokens over 8k keys, 16/2 heads of 128; 319 GFLOP): 305 us in a short burst at 1.83 GHz, 354 us
-//     over 0.15 s of launches, when the power limit brings the clock to 1.6 GHz: 900-1 050 TFLOP/s.  Tensor pipe and
-//     exponential unit are both at 0.5; a softmax group takes 2 030 cycles for 64 keys and never waits.  Tried: sixteen
+//   long prompts (6.8k new tokens over 8k keys, 16/2 heads of 128; 319 GFLOP): 323 us in bursts at 1.97 GHz, 337-348
+//     us when the power limit brings the clock to 1.7 GHz: 920-990 TFLOP/s.  Tensor pipe and
+//     exponential unit are both at 0.5; a softmax group takes some 2 000 cycles for 64 keys and never waits.  Tried: sixteen
 //     softmax warps (one group per stream and half), one softmax step per 128 keys with the issue in strict turns,
 //     part of the exponentials as a cubic on the FMA pipe: none is faster over long blocks.
-//   decode (64 sequences, window 4 096, 177 MB): 41 us in a graph, 4.3 TB/s; from the first tile (4 us after the launch) to
+//   decode (64 sequences, window 4 096, 177 MB): 40 us in a graph, 4.4 TB/s; from the first tile (4 us after the launch) to
 //     the last (33 us) the keys stream at 0.9 of the copy rate, the rest is start, drain and joining of cut units.
-//   one token, 1 028 keys: 9.3 us, of which the last piece's joining is 2 and fence and ticket 1.  A half tile in which no
-//     row sees a key (behind the last one) is left out: 10.4 without that, five drafted tokens of each of 8 sequences
-//     14.2 instead of 15.5 (a first pass over the softmax costs 1.4).
+//   one token, 1 028 keys: 9.0 us, of which the last piece's joining is 2 and fence and ticket 1.  Five drafted tokens of
+//     each of 8 sequences: 13.2.  A half tile in which no row sees a key (behind the last one) is left out, 1.1 us of either.
 //
 // TMEM columns (512): halves 0, 1 of S_0/P_0 [0,64) [64,128), of S_1/P_1 [128,192) [192,256), O_0 [256,384)  O_1 [384,512).
 #include <algorithm>
@@ -89,7 +88,7 @@ constexpr uint32_t kMaxLen = kChunkMaxLen;
 constexpr uint32_t kTile = kChunkTile;
 constexpr uint32_t kThreads = 384;
 constexpr uint32_t kProducerWarp = 8, kIssuerWarp = 9, kQWarp = 11;
-constexpr uint64_t kWaitNs = 2000000000ull;  // bits of the status word: the `code` of the wait that ran out (kStatusBadPage is none of them)
+constexpr uint64_t kWaitNs = 2000000000ull;  // a wait that takes longer sets its bit of the status word and gives up
 constexpr float kNegInf = -1e30f;  // a row's maximum before its first key
 // Products of f16 rows of 128 are below 2^39: with this scale every finite score stays above kNegInf.
 constexpr float kMaxScale = 1e18f;

@@ -10,9 +10,9 @@
 // chunks at a time (append.cuh), several in flight.  V bytes of the 8-bit cache are transposed through shared memory: a
 // whole block goes out as 16-byte words, a part of one byte by byte.
 //
-// Measured: 8.2k tokens of 32/8 heads of 128 (210 MB) 39.6 us, 5.3 TB/s, 0.81 of the copy rate; 6.1k tokens of 16/2 heads
+// Measured: 8.5k tokens of 32/8 heads of 128 (210 MB) 39.4 us, 5.3 TB/s, 0.81 of the copy rate; 4.8k tokens of 16/2 heads
 // into the 8-bit cache (47 MB) 17 us - two thirds of it launch, the chain of loads before a CTA's first row (sequence,
-// page, positions, tables) and the drain; one token of each of 64 sequences 3.5 us.
+// page, positions, tables) and the drain; one token of each of 64 sequences 3.3 us.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -287,8 +287,8 @@ mf_status launch_mrope(MfContext *ctx, MropeParams &p, const char *what)
     const uint32_t R = K8 ? 16 : 8, cpr = p.head_dim / 16;
     const uint64_t blocks = first_block(p.tokens, p.batch, R) + 1;
     const uint64_t slots = (p.q_rot ? p.n_heads : 0) + (uint64_t)(K8 ? 1 : 2) * p.n_kv_heads;
-    // Prompts: so many parts that a whole block leaves every thread two rounds of loads (one round: 41 and 18 us for 8.2k
-    // tokens of 32/8 heads and 6.1k tokens into the 8-bit cache, two: 39.6 and 17, no parts at all: 57 and 26).  Decode
+    // Prompts: so many parts that a whole block leaves every thread two rounds of loads (one round: 41 and 18 us for 8.5k
+    // tokens of 32/8 heads and 4.8k tokens into the 8-bit cache, two: 39.6 and 17, no parts at all: 57 and 26).  Decode
     // steps (a token or few per sequence) have little for a CTA as it is.
     const uint64_t per_part = 2ull * in_flight(K8) * kThreads;
     uint64_t parts = 1;

@@ -12,7 +12,8 @@ namespace {
 // Costs in a common unit of about a quarter of a microsecond: a tile of a unit with more than 128 rows (two query tiles on
 // every key tile: 2.3 us, the softmax's pace), a tile of a unit with at most that (1.4 us, the memory's pace), and what
 // an item costs its CTA beyond its tiles (q, draining the products, writing the rows, joining: about 4 us).  With equal
-// costs for all tiles the CTAs that had a mixed step's prompt rows ended 90 us behind the others.
+// costs for all tiles the CTAs that had a mixed step's prompt rows ended 90 us behind the others.  Measured at head_dim 128
+// and used for 64, too, where a tile has half the bytes and the same exponentials.
 constexpr uint32_t kRowsTileCost = 9, kKeysTileCost = 5, kItemCost = 16;
 // Shortest piece a unit is cut into when every CTA has several units, in tiles.
 constexpr uint32_t kMinPiece = 2;
