@@ -41,8 +41,8 @@
 //     part of the exponentials as a cubic on the FMA pipe: none is faster over long blocks.
 //   decode (64 sequences, window 4 096, 177 MB): 40 us in a graph, 4.4 TB/s; from the first tile (4 us after the launch) to
 //     the last (33 us) the keys stream at 0.9 of the copy rate, the rest is start, drain and joining of cut units.
-//   one token, 1 028 keys: 9.0 us, of which the last piece's joining is 2 and fence and ticket 1.  Five drafted tokens of
-//     each of 8 sequences: 13.2.  A half tile in which no row sees a key (behind the last one) is left out, 1.1 us of either.
+//   one token, 1 028 keys: 9.0-10.0 us, of which the last piece's joining is 2 and fence and ticket 1.  Five drafted tokens of
+//     each of 8 sequences: 13.2-13.9.  A half tile in which no row sees a key (behind the last one) is left out, 1.1 us of either.
 //
 // TMEM columns (512): halves 0, 1 of S_0/P_0 [0,64) [64,128), of S_1/P_1 [128,192) [192,256), O_0 [256,384)  O_1 [384,512).
 #include <algorithm>
@@ -215,6 +215,22 @@ __device__ __noinline__ float far_weights(uint32_t tm, const Visible vis, int32_
         tmem_st16(tm + c * 16, pk);
     }
     return sum;
+}
+
+// Means of f16 values stay in f16's range: the rounding of the weights (2^-11 of each) can carry one past its end, where the
+// rounding to f16 would make it an infinity.  (0.06 us of a small call, 2 % of window 512 prompts; a look at the packed words
+// and a second pass over TMEM for the rows that need it cost the same and more.)
+template <uint32_t N>
+__device__ __forceinline__ void keep_inside(float (&o)[N])
+{
+    float top = 0.f;
+#pragma unroll
+    for (uint32_t q = 0; q < N; q += 2) top = max3(top, fabsf(o[q]), fabsf(o[q + 1]));
+    if (top > 65504.f) {
+#pragma unroll
+        for (uint32_t q = 0; q < N; ++q)
+            if (fabsf(o[q]) < 65600.f) o[q] = fminf(fmaxf(o[q], -65504.f), 65504.f);
+    }
 }
 
 // Columns of a unit's page list by who sees them.  [gap0, gap1) and what lies behind `end`: no row.  [sink0, sink1),
@@ -798,6 +814,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                         }
                         continue;
                     }
+                    keep_inside(o);
                     uint32_t w[16];
 #pragma unroll
                     for (uint32_t q = 0; q < 16; ++q) w[q] = pack_f16x2(o[2 * q], o[2 * q + 1]);
@@ -882,9 +899,12 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                         uint4 *to = reinterpret_cast<uint4 *>(p.out + (it.tok0 + (uint64_t)tk) * p.out_stride_t +
                                                               (uint64_t)(it.kvh * G + row - tk * G) * p.out_stride_h + grp * 16);
 #pragma unroll
+                        for (uint32_t e = 0; e < 16; ++e) o[e] *= inv;
+                        keep_inside(o);
+#pragma unroll
                         for (uint32_t e = 0; e < 2; ++e)
-                            to[e] = make_uint4(pack_f16x2(o[8 * e] * inv, o[8 * e + 1] * inv), pack_f16x2(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
-                                               pack_f16x2(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack_f16x2(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+                            to[e] = make_uint4(pack_f16x2(o[8 * e], o[8 * e + 1]), pack_f16x2(o[8 * e + 2], o[8 * e + 3]),
+                                               pack_f16x2(o[8 * e + 4], o[8 * e + 5]), pack_f16x2(o[8 * e + 6], o[8 * e + 7]));
                     }
                 }
                 named_bar_sync(9, 256);  // words[kLast] and the partial rows are free again

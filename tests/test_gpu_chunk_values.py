@@ -225,3 +225,27 @@ def test_large_scores(mfk, foundry, size, q_lens, kv_lens):
                 tol = 2.0 ** -25 + 2.0 ** -11 * want.abs() + (2.0 ** -11 + 2.0 ** -12) * mean
                 assert bool(((got[t:t + nq, h] - want).abs() <= tol).all())
             t += nq
+
+
+@pytest.mark.parametrize("value", [65504.0, -65504.0])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("q_len,n,page", [(1, 201, 16), (1, 6001, 64), (30, 230, 16), (30, 6001, 128)])
+def test_means_stay_in_the_range(mfk, foundry, value, d, q_len, n, page):
+    """Weights that all round up (0.6 of a step of f16 above one half) carry a mean of f16's largest values past it."""
+    case = ChunkCase(hq=8, hkv=1, d=d, page=page, q_lens=[q_len], kv_lens=[n])
+    case.q.zero_()
+    case.q.view(-1, 8, d)[..., :2] = 1.0
+    score = float(torch.log(torch.tensor(0.5 * (1 + 0.6 * 2.0 ** -10), dtype=torch.float64)))
+    first = float(torch.tensor(score).half())
+    for page_id in case.table[0].tolist():
+        case.k[page_id].zero_()
+        case.k[page_id, :, :, 0], case.k[page_id, :, :, 1] = first, score - first
+        case.v[page_id] = value
+    case.k[int(case.table[0, 0]), :, 0, :2] = 0  # the one with weight 1
+    out = torch.empty_like(case.q)
+    plan = case.plan(foundry)
+    foundry.paged_chunk_attention(plan, case.cache(mfk), case.q, out, scale=1.0)
+    foundry.synchronize()
+    # the weights are off by 2^-11 of each, f32 sums by 2^-12
+    assert bool(torch.isfinite(out).all()) and bool(((out.double() - value).abs() <= 2.0 ** -10 * 65504).all())
+    plan.close()
